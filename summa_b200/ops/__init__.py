@@ -11,12 +11,13 @@ from typing import Optional
 
 import torch
 
-from . import reference
+from . import paged, reference
+from .paged import PagedKV, PagedRows
 from .reference import rope_table as _rope_table_ref
 
 __all__ = [
     "linear", "rmsnorm", "add_rmsnorm", "layernorm", "rope_table", "qk_norm_rope", "attention",
-    "attention_dropout", "kv_append", "conv1d_silu", "selective_scan", "mul_silu", "gated_act",
+    "attention_dropout", "kv_append", "PagedKV", "PagedRows", "paged_append", "paged_attention", "conv1d_silu", "selective_scan", "mul_silu", "gated_act",
     "activation", "router_logits", "moe_route", "moe_aux_loss", "moe_experts", "embedding",
     "linear_cross_entropy", "reference", "set_backend", "backend", "native_enabled",
 ]
@@ -155,6 +156,43 @@ def kv_append(k_cache, v_cache, k, v, offset):
     S = k.shape[1]
     k_cache[:, offset:offset + S].copy_(k)
     v_cache[:, offset:offset + S].copy_(v)
+
+
+def paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv: PagedKV, rows: PagedRows, out=None):
+    """`packed_qk_rope` for sequences of different lengths, with the keys and values going into the paged cache `kv`: the rows
+    `[T, (Hq + 2 Hkv) * D]` get their optional QK-norm and their rotation at the position that each has in its sequence
+    (`rows.lengths[b]` + its number there). Returns the queries `[T, Hq, D]` (in `out` when given).
+
+    In 8 bits the rows that this call puts into a page and head need a scale of at least their largest magnitude / 448, as a power of
+    two; the page's first slot begins the scale anew, otherwise it only grows, and the codes in front of the rows are then rounded
+    to the new one. An infinite or NaN element is stored as NaN and does not count for the scale. Rows of a slot that is not in use store
+    nothing and return zeros; rows behind the last sequence are zeros, or as they were in `out`. No two sequences of a call may append
+    to one page. A position without a page (or beyond cos / sin) stores nothing and returns zeros on CUDA, and sets bit 4 of the device's error
+    word (`native.read_error_flag`); on the CPU it raises. No gradients."""
+    paged.check_append(qkv, q_gamma, k_gamma, cos, sin, Hq, Hkv, D, kv, rows, out)
+    _no_gradient("paged_append", qkv, q_gamma, k_gamma)
+    if native_enabled(qkv) and D in (64, 128):
+        return _cu().paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv, rows, out)
+    return paged.append_reference(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv, rows, out)
+
+
+def paged_attention(q, kv: PagedKV, rows: PagedRows, causal=True, window=None, scale=None, out=None):
+    """Attention of the rows `[T, Hq, D]` over the paged cache, which holds them already (`paged_append` with the same `rows`): row
+    i of sequence b stands at lengths[b] + i and sees its sequence's keys up to there (all of them with `causal=False`), within `window`
+    on either side. Returns `[T, Hq, D]` (in `out` when given); rows that see no key, and those of a slot that is not in use, are
+    zeros, rows behind the last sequence zeros, or as they were in `out`. Keys without a page are left out on CUDA, and set bit 4 of the
+    device's error word; on the CPU they raise. A value that is not finite reaches the rows whose sequence holds it, and no others; within
+    the rows of one call it may also reach those that the mask keeps from it. No gradients."""
+    paged.check_attention(q, kv, rows, window, out)
+    _no_gradient("paged_attention", q)
+    if native_enabled(q) and q.shape[2] in (64, 128):
+        return _cu().paged_attention(q, kv, rows, causal, window, scale, out)
+    return paged.attention_reference(q, kv, rows, causal, window, scale, out)
+
+
+def _no_gradient(name, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
 
 
 def conv1d_silu(x, weight, bias, state=None):

@@ -1,0 +1,90 @@
+// What the kernels of the paged key/value cache share: the description of a cache and of a batch, and the 8-bit element.
+//
+// A cache layer holds its keys and its values in pages `[num_pages, Hkv, page, D]` (the rows of one page and head lie together,
+// so that a head's block of keys is one contiguous piece). In 8 bits an element is an e4m3 code times the scale of its page and
+// head, a power of two: dividing by it, and moving codes to a larger one, is exact but for codes that fall below the type's
+// smallest step, and an e4m3 value is as precise at any scale, so nothing is lost against a scale of full precision.
+//
+// Sequence b has `lengths[b]` tokens in the cache before the call (negative: a slot that is not in use) and brings the rows
+// `starts[b] .. starts[b + 1]` of the call (row b without `starts`); row i of it stands at position lengths[b] + i. Position p
+// lives in page table[b][p / page], slot p % page. Everything that is read on the device is taken as it may come: row ranges are
+// cut to the call's rows, and a position without a valid page is reported in the error word (bit 4) and skipped.
+#pragma once
+#include "host_util.h"
+#include "sm100.cuh"
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+namespace sb {
+
+constexpr int PAGED_LEAST_EXP = -60, PAGED_MOST_EXP = 120;   // range of log2(scale)
+constexpr int PAGED_MAX_PAGE = 128;
+
+struct PagedBatch {
+  const int* table;          // [B, P], row stride table_ld
+  const int* lengths;        // [B]
+  const int* starts;         // [B + 1] or null
+  long table_ld;
+  int P, B, T, max_rows;
+  int page_shift, num_pages;
+};
+
+struct PagedSeq {
+  int row0, rows;            // the rows of the call that are its own
+  int len;                   // tokens in the cache before the call, < 0: not in use
+};
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& p, int b) {
+  PagedSeq s;
+  s.len = p.lengths[b];
+  if (p.starts == nullptr) {
+    s.row0 = b;
+    s.rows = 1;
+  } else {
+    s.row0 = min(max(p.starts[b], 0), p.T);
+    s.rows = min(max(p.starts[b + 1], s.row0), p.T) - s.row0;
+  }
+  return s;
+}
+
+// First row behind the last sequence.
+__device__ __forceinline__ int paged_tail(const PagedBatch& p) {
+  return p.starts == nullptr ? p.T : min(max(p.starts[p.B], 0), p.T);
+}
+
+// Page of position `pos` (>= 0) of sequence b, -1 if there is none.
+__device__ __forceinline__ int paged_page(const PagedBatch& p, int b, long pos) {
+  const long i = pos >> p.page_shift;
+  if (i >= p.P) return -1;
+  const int id = p.table[b * p.table_ld + i];
+  return static_cast<unsigned>(id) < static_cast<unsigned>(p.num_pages) ? id : -1;
+}
+
+// log2 of a scale, which is a power of two.
+__device__ __forceinline__ int scale_exp(float s) { return static_cast<int>((__float_as_uint(s) >> 23) & 255u) - 127; }
+__device__ __forceinline__ float exp_scale(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// The smallest e in the range with most <= 448 * 2^e (448 = 1.75 * 2^8): from the bits of `most`, no logarithm that could round.
+__device__ __forceinline__ int e4m3_exp(float most) {
+  const uint32_t u = __float_as_uint(most);
+  const int e = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return min(max(e, PAGED_LEAST_EXP), PAGED_MOST_EXP);
+}
+
+// Two values to two e4m3 codes (the first in the low byte): nearest, ties to even, NaN for NaN. Infinities come as NaN from the
+// caller: the conversion itself would make the largest finite value of them.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t v) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v), __NV_E4M3);
+  return __half22float2(__half2(h));
+}
+
+// Host: log2 of a page size, -1 if it is not one that the kernels take.
+inline int page_shift_of(int page) {
+  return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1;
+}
+
+}  // namespace sb

@@ -9,6 +9,7 @@ place by the GEMM epilogue and receive `None` from autograd.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import math
 from typing import Optional, Tuple
@@ -578,6 +579,88 @@ def decode_attention(q, k, v, causal, window, q_offset, scale=None):
     N.call("sb_attention_decode", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ws.data_ptr(), B, Hq, Hkv, Sk,
            cap, D, qs, _bshd_strides(k), _bshd_strides(v), os_, float(scale), splits, N.stream())
     return o
+
+
+N.register("sb_paged_append", [N.P] * 13 + [N.I] * 11 + [N.F] + [N.L] * 9 + [N.P])
+N.register("sb_paged_attention", [N.P] * 10 + [N.I] * 12 + [N.F] + [N.L] * 11 + [N.P])
+N.register("sb_paged_attention_workspace", [N.I] * 7, restype=ctypes.c_long)
+
+
+def _cache_strides(kv):
+    """(k page, k head, v page, v head, k_scale page, v_scale page) in elements."""
+    k, v, ks, vs = kv
+    a, b = k.stride(), v.stride()
+    return a[0], a[1], b[0], b[1], 0 if ks is None else ks.stride(0), 0 if vs is None else vs.stride(0)
+
+
+def _heads_ok(t: torch.Tensor) -> bool:
+    """Rows of heads `[T, H, D]` whose heads begin on 16 bytes."""
+    s = t.stride()
+    return s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0
+
+
+def paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv, rows, out=None):
+    """See `ops.paged_append`."""
+    if qkv.device.index != torch.cuda.current_device():
+        with torch.cuda.device(qkv.device):
+            return paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv, rows, out)
+    T = qkv.shape[0]
+    if out is not None and not (_heads_ok(out) and out.stride(1) == D):
+        q = out.contiguous()
+        q = q.clone() if q.data_ptr() % 16 else q
+    else:
+        q = torch.empty(T, Hq, D, device=qkv.device, dtype=BF16) if out is None else out
+    if T > 0:
+        x, ld = _rows(qkv)
+        qg, kg = (None, None) if q_gamma is None else (_gains(q_gamma), _gains(k_gamma))
+        k, v, ks, vs = kv
+        table, lengths, starts, _ = rows
+        N.call("sb_paged_append", x.data_ptr(), q.data_ptr(), N.ptr(qg), N.ptr(kg), N.ptr(cos), N.ptr(sin), k.data_ptr(), v.data_ptr(),
+               N.ptr(ks), N.ptr(vs), table.data_ptr(), lengths.data_ptr(), N.ptr(starts), T, table.shape[0], table.shape[1], Hq, Hkv, D,
+               k.shape[2], k.shape[0], cos.shape[0] if cos is not None else 0, rows.most(T), 1 if out is None else 0, eps, ld, q.stride(0),
+               table.stride(0), *_cache_strides(kv), N.stream())
+    if out is not None and q is not out:
+        out.copy_(q)
+    return q if out is None else out
+
+
+def _gains(g: torch.Tensor) -> torch.Tensor:
+    """fp32, contiguous and on 16 bytes."""
+    g = _gamma32(g).contiguous()
+    return g.clone() if g.data_ptr() % 16 else g
+
+
+@functools.lru_cache(maxsize=256)
+def _paged_workspace(device, B, Hkv, P, page, D, fp8, columns):
+    return N.call_value("sb_paged_attention_workspace", B, Hkv, P, page, D, fp8, columns)
+
+
+def paged_attention(q, kv, rows, causal=True, window=None, scale=None, out=None):
+    """See `ops.paged_attention`."""
+    device = q.device.index
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return paged_attention(q, kv, rows, causal, window, scale, out)
+    T, Hq, D = q.shape
+    q = q if _heads_ok(q) else q.clone(memory_format=torch.contiguous_format)
+    if out is not None and not _heads_ok(out):
+        o = out.clone(memory_format=torch.contiguous_format)
+    else:
+        o = torch.empty(T, Hq, D, device=q.device, dtype=BF16) if out is None else out
+    if T > 0:
+        k, v, ks, vs = kv
+        table, lengths, starts, _ = rows
+        pages, Hkv, page, _ = k.shape
+        B, P = table.shape
+        most, fp8 = rows.most(T), 0 if ks is None else 1
+        ws = torch.empty(_paged_workspace(device, B, Hkv, P, page, D, fp8, most * (Hq // Hkv)), device=q.device, dtype=torch.float32)
+        N.call("sb_paged_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), N.ptr(ks), N.ptr(vs), o.data_ptr(), ws.data_ptr(),
+               table.data_ptr(), lengths.data_ptr(), N.ptr(starts), T, B, P, Hq, Hkv, D, page, pages, most, 1 if causal else 0,
+               -1 if window is None else min(int(window), 0x7fffffff), 1 if out is None else 0, 1.0 / math.sqrt(D) if scale is None else scale,
+               table.stride(0), q.stride(0), q.stride(1), o.stride(0), o.stride(1), *_cache_strides(kv), N.stream())
+    if out is not None and o is not out:
+        out.copy_(o)
+    return o if out is None else out
 
 
 class _PackedAttention(torch.autograd.Function):
