@@ -118,6 +118,7 @@ __device__ __forceinline__ int grown_exp(float old, int slot, float most, float*
 template <int D, bool FP8>
 __global__ void __launch_bounds__(256) paged_append_rows_kernel(const AppendParams p) {
   constexpr int TPH = D / 8;
+  asm volatile("griddepcontrol.launch_dependents;");
   const int heads = p.Hq + 2 * p.Hkv;
   const long item = (blockIdx.x * 256L + threadIdx.x) / TPH;
   const int part = threadIdx.x % TPH;
@@ -196,6 +197,7 @@ template <int D, int NP>
 __global__ void __launch_bounds__(256) paged_append_segments_kernel(const AppendParams p) {
   constexpr int TPH = D / 8, RPP = 256 / TPH;        // threads of a row, rows of a pass
   __shared__ float red[8];
+  asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int shift = p.batch.page_shift, page_rows = 1 << shift;
   // every warp finds the segment by itself: segments of 32 sequences at a time, summed over the lanes

@@ -43,15 +43,14 @@ struct PagedAttnParams {
   int causal, window;               // window < 0: none
   float scale_log2;
   int zero_tail;
-  float* part;                      // partials: [2 * CTAs][columns][D] of O, then [2 * CTAs][columns][2] of (m, l)
+  float* part;                      // partials: [2 * CTAs] of O, then [2 * CTAs][columns][2] of (m, l)
   int ctas;
   unsigned int* err;
 };
 
-#ifndef PD_CTAS
-#define PD_CTAS 2
-#endif
-constexpr int PD_WARPS = 4, PD_STAGE = 8192, PD_START = 2;
+constexpr int PD_WARPS = 4, PD_STAGE = 8192, PD_NS = 3;   // a warp's ring: stages of keys and values
+constexpr int PD_START = 3;                               // what a (sequence, kv head) costs beside its keys, in units
+constexpr int PD_WHOLE = 5;                               // up to so many units it is not worth a cut and the joining kernel
 template <int D, bool FP8> struct PagedDecode {
   static constexpr int ROW = FP8 ? D : 2 * D;                 // bytes of a key
   static constexpr int KT = PD_STAGE / 2 / ROW;               // keys of a warp's tile: 16, 32 or 64
@@ -90,58 +89,68 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnParams& p, int b)
   return r;
 }
 
-// The list that is cut into stretches: every (sequence, kv head) counts as its units and PD_START more for its beginning and end.
-template <int UNIT>
-__device__ __forceinline__ int paged_length(const PagedAttnParams& p, int b) {
-  const int u = paged_span<UNIT>(p, b).units;
-  return u > 0 ? (u + PD_START) * p.Hkv : 0;
-}
-template <int UNIT>
-__device__ __forceinline__ int paged_total(const PagedAttnParams& p, int lane) {
-  int n = 0;
-  for (int b = lane; b < p.batch.B; b += 32) n += paged_length<UNIT>(p, b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n;
-}
+// How the list of (sequence, kv head) is cut: places [begin(c), begin(c + 1)) are stretch c, equal ones, the first of them longer by one
+// where it does not divide. Each counts as its units and PD_START more for its beginning and end; but where all of them are short
+// (PD_WHOLE units at most) each is one place, and nothing is cut.
+struct Stretches {
+  int share, more;
+  bool whole;
+  __device__ __forceinline__ int length(int units) const { return units <= 0 ? 0 : whole ? 1 : units + PD_START; }
+  __device__ __forceinline__ int begin(int c) const { return c * share + min(c, more); }
+  // the stretch that place x lies in
+  __device__ __forceinline__ int of(int x) const {
+    const int longer = more * (share + 1);
+    return x < longer ? x / (share + 1) : more + (x - longer) / share;    // (share is 0 only if all places lie in the longer ones)
+  }
+};
 
-// The sequence that place `at` of the list belongs to (B behind the end); *before: the length of those in front of it.
+// Cuts the list into `ctas` stretches and finds the sequence at the beginning of stretch c (B behind the end of the list); *at: that
+// place, *before: the places in front of the sequence. By a whole warp.
 template <int UNIT>
-__device__ __forceinline__ int paged_find(const PagedAttnParams& p, int at, int* before, int lane) {
-  int sum0 = 0;
-  for (int b0 = 0; b0 < p.batch.B; b0 += 32) {
-    const int n = b0 + lane < p.batch.B ? paged_length<UNIT>(p, b0 + lane) : 0;
+__device__ __forceinline__ int paged_locate(const PagedAttnParams& p, int c, int ctas, Stretches* cut, int* at, int* before) {
+  const int lane = threadIdx.x & 31, B = p.batch.B;
+  int units = lane < B ? paged_span<UNIT>(p, lane).units : 0;
+  int all = units, some = units > 0, most = units;
+  for (int b = lane + 32; b < B; b += 32) {
+    const int u = paged_span<UNIT>(p, b).units;
+    all += u; some += u > 0; most = max(most, u);
+  }
+  cut->whole = __reduce_max_sync(0xffffffffu, most) <= PD_WHOLE;
+  const int total = __reduce_add_sync(0xffffffffu, cut->whole ? some : all + some * PD_START) * p.Hkv;
+  cut->share = total / ctas;
+  cut->more = total - cut->share * ctas;
+  *at = cut->begin(c);
+  int front = 0;
+  for (int b0 = 0;;) {
+    const int n = cut->length(units) * p.Hkv;
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += x;
     }
-    const int all = __shfl_sync(0xffffffffu, sum, 31);
-    if (at < sum0 + all) {
-      const int l = __popc(__ballot_sync(0xffffffffu, sum0 + sum <= at));
-      *before = sum0 + __shfl_sync(0xffffffffu, sum - n, l);
+    const unsigned in_front = __ballot_sync(0xffffffffu, front + sum <= *at);
+    if (in_front != 0xffffffffu) {
+      const int l = __popc(in_front);
+      *before = front + __shfl_sync(0xffffffffu, sum - n, l);
       return b0 + l;
     }
-    sum0 += all;
+    front += __shfl_sync(0xffffffffu, sum, 31);
+    if ((b0 += 32) >= B) break;
+    units = b0 + lane < B ? paged_span<UNIT>(p, b0 + lane).units : 0;
   }
-  *before = sum0;
-  return p.batch.B;
+  *before = front;
+  return B;
 }
-
-// Stretch c of the list is [begin(c), begin(c + 1)): equal ones, the first of them longer by one where it does not divide.
-struct Stretches {
-  int share, more;
-  __device__ __forceinline__ Stretches(int total, int ctas) : share(total / ctas), more(total % ctas) {}
-  __device__ __forceinline__ int begin(int c) const { return c * share + min(c, more); }
-};
 
 // Where a CTA (or a warp's copies, running ahead) is in its stretch: units [u, u_end) of (b, kh), nothing left when they are empty.
 template <int UNIT>
 struct PagedWalk {
   PagedSpan s;
   int b, kh, u, u_end, left;
+  bool whole;
   __device__ __forceinline__ void enter(int x) {
+    if (whole) { --left; u = 0; u_end = s.units; return; }
     const int end = min(s.units + PD_START, x + left);
     left -= end - x;
     u = max(x - PD_START, 0);
@@ -160,16 +169,18 @@ struct PagedWalk {
       enter(0);
     }
   }
-  __device__ __forceinline__ void start(const PagedAttnParams& p, int begin, int end, int lane) {
-    left = end - begin;
-    b = kh = u = u_end = 0;
-    if (left <= 0) return;
-    int before;
-    b = paged_find<UNIT>(p, begin, &before, lane);
-    if (b >= p.batch.B) { left = 0; return; }
+  __device__ __forceinline__ void start(const PagedAttnParams& p, int c, int ctas) {
+    Stretches cut;
+    int at, before;
+    b = paged_locate<UNIT>(p, c, ctas, &cut, &at, &before);
+    left = cut.begin(c + 1) - at;
+    whole = cut.whole;
+    kh = u = u_end = 0;
+    if (left <= 0 || b >= p.batch.B) { left = 0; return; }
     s = paged_span<UNIT>(p, b);
-    kh = (begin - before) / (s.units + PD_START);
-    enter((begin - before) % (s.units + PD_START));
+    const int length = cut.length(s.units);
+    kh = (at - before) / length;
+    enter(at - before - kh * length);
     if (u == u_end) next(p);
   }
 };
@@ -215,43 +226,63 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// CTAs to an SM, and the stages of a warp's ring that fit beside each other then.
-template <int NT> struct PagedShape { static constexpr int CTAS = NT == 1 ? PD_CTAS : 2, NS = CTAS == 2 ? 3 : 2; };
+// The first of the two dimensions that accumulator quad d of a thread of group g holds.
+template <int D, bool FP8>
+__device__ __forceinline__ int paged_dim(int g, int d) {
+  return !FP8 && D == 128 ? 64 * (d >> 2) + 8 * g + 2 * (d & 3) : (D / 8) * g + 2 * d;
+}
+
+// Shared memory: the rings; per stage 64 bytes of scales and page ids; two warps' O and all warps' (m, l) where they meet.
 template <int D, int NT> constexpr int paged_decode_smem() {
-  return PD_WARPS * PagedShape<NT>::NS * (PD_STAGE + 64) + 16 * D * 4 + 2 * PD_WARPS * 8 * NT * 2 * 4;
+  return PD_WARPS * PD_NS * (PD_STAGE + 64) + (NT == 1 ? 2 : 1) * 8 * NT * D * 4 + 2 * PD_WARPS * 8 * NT * 2 * 4;
 }
 
 // NT column tiles of 8.
 template <int D, bool FP8, int NT>
-__global__ void __launch_bounds__(PD_WARPS * 32, PagedShape<NT>::CTAS)
+__global__ void __launch_bounds__(PD_WARPS * 32, 2)
 paged_decode_kernel(const PagedAttnParams p) {
   using C = PagedDecode<D, FP8>;
-  constexpr int NS = PagedShape<NT>::NS, KT = C::KT, MT = C::MT, UNIT = C::UNIT, ROW = C::ROW, COLS = 8 * NT, MD = D / 16, KSTEPS = D / 16;
-  constexpr int RB = 2 / NT;                             // warps that put their O down at a time
+  constexpr int NS = PD_NS, KT = C::KT, MT = C::MT, UNIT = C::UNIT, ROW = C::ROW, COLS = 8 * NT, MD = D / 16, KSTEPS = D / 16;
+  constexpr int RB = NT == 1 ? 2 : 1;                    // warps that put their O down at a time (two CTAs have to fit an SM)
+  constexpr int QUADS = NT * MD;                         // accumulators of a thread, in fours
   constexpr float HEAD = FP8 ? 11.f : 0.f, SLACK = FP8 ? 4.f : 8.f;
   extern __shared__ __align__(128) uint8_t smem[];
-  asm volatile("griddepcontrol.launch_dependents;");
+  // Nothing is read before the wait, and the joining kernel, which reads the batch's description before its own, starts after it.
+  asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * (NS * PD_STAGE);
   // per stage: [4] key scales, [4] value scales, [4] page ids of the tile's groups of 16 keys, [1] whether it has all its keys
   uint8_t* meta = smem + PD_WARPS * NS * PD_STAGE + warp * (NS * 64);
-  float* red_o = reinterpret_cast<float*>(smem + PD_WARPS * NS * (PD_STAGE + 64));         // [RB][COLS][D]
-  float* red_ml = red_o + 16 * D;                                                          // [2][PD_WARPS][COLS][2]
+  float4* red_o = reinterpret_cast<float4*>(smem + PD_WARPS * NS * (PD_STAGE + 64));       // [RB][QUADS][32]
+  float* red_ml = reinterpret_cast<float*>(red_o + RB * QUADS * 32);                       // [2][PD_WARPS][COLS][2]
 
-  if (p.zero_tail) {
-    const int t0 = paged_tail(p.batch);
-    const long n = static_cast<long>(p.batch.T - t0) * p.Hq * (D / 8);
-    for (long i = blockIdx.x * (PD_WARPS * 32L) + threadIdx.x; i < n; i += gridDim.x * (PD_WARPS * 32L)) {
-      const long row = i / (p.Hq * (D / 8));
-      const int x = static_cast<int>(i % (p.Hq * (D / 8)));
-      *reinterpret_cast<uint4*>(p.o + (t0 + row) * p.o_ld + (x / (D / 8)) * p.o_head + (x % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
-    }
-  }
-
-  const Stretches cut(paged_total<UNIT>(p, lane), gridDim.x);
   PagedWalk<UNIT> cur, ahead;
-  cur.start(p, cut.begin(blockIdx.x), cut.begin(blockIdx.x + 1), lane);
+  cur.start(p, blockIdx.x, gridDim.x);
   ahead = cur;
+
+  // The query columns as they lie, operand B of S^T in the order of the elements that a thread loads of a key. Those of the first (sequence,
+  // kv head) are asked for before its keys.
+  uint32_t qf[NT][KSTEPS][2];
+  auto load_q = [&]() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int c = n * 8 + g;
+      const __nv_bfloat16* src = p.q + (cur.s.row0 + c / p.G) * p.q_ld + (cur.kh * p.G + c % p.G) * p.q_head;
+      const bool there = cur.u < cur.u_end && c < cur.s.rows * p.G;
+#pragma unroll
+      for (int j = 0; j < C::LOADS; ++j) {
+        const int chunk = C::LOADS == 1 ? t : C::LOADS == 2 ? 2 * t + j : 2 * t + (j & 1) + 8 * (j >> 1);
+#pragma unroll
+        for (int k = 0; k < C::EPC / 8; ++k) {
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (there) w = *reinterpret_cast<const uint4*>(src + chunk * C::EPC + 8 * k);
+          const int at = j * (C::EPC / 4) + 2 * k;
+          qf[n][at][0] = w.x; qf[n][at][1] = w.y; qf[n][at + 1][0] = w.z; qf[n][at + 1][1] = w.w;
+        }
+      }
+    }
+  };
+  load_q();
 
   // The warp's copies of its next tile: KT rows of keys, then of values, zeros where the sequence has no key. The pages are looked up
   // one tile ahead of their copies.
@@ -277,7 +308,7 @@ paged_decode_kernel(const PagedAttnParams p) {
       bool all = key0 >= ahead.s.lo && key0 + KT <= ahead.s.hi;
 #pragma unroll
       for (int m = 0; m < MT; ++m) all = all && static_cast<unsigned>(id[m]) < static_cast<unsigned>(p.batch.num_pages);
-      if (all) {
+      if (__builtin_expect(all, 1)) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           const uint32_t off = ((key0 + m * 16) & mask) * ROW + lane * 16;
@@ -289,7 +320,7 @@ paged_decode_kernel(const PagedAttnParams p) {
             cp_async16(at + KT * ROW, vsrc + i * 512);
           }
         }
-      } else {
+      } else {                                         // (an edge of the sequence, or a page that is none)
 #pragma unroll 1
         for (int m = 0; m < MT; ++m) {
           int page = -2;
@@ -323,39 +354,34 @@ paged_decode_kernel(const PagedAttnParams p) {
           cp_async4(smem_u32(at + 16), p.vs + (good ? page * p.vs_ld + ahead.kh : 0));
         }
       }
-      if (++ahead.u == ahead.u_end) ahead.next(p);
+      if (__builtin_expect(++ahead.u == ahead.u_end, 0)) ahead.next(p);
       look_up();
     }
     cp_async_commit();
     put = put + 1 == NS ? 0 : put + 1;
   };
   look_up();
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < NS - 1; ++i) fetch();
+
+  if (p.zero_tail) {
+    const int t0 = paged_tail(p.batch);
+    const long n = static_cast<long>(p.batch.T - t0) * p.Hq * (D / 8);
+    for (long i = blockIdx.x * (PD_WARPS * 32L) + threadIdx.x; i < n; i += gridDim.x * (PD_WARPS * 32L)) {
+      const long row = i / (p.Hq * (D / 8));
+      const int x = static_cast<int>(i % (p.Hq * (D / 8)));
+      *reinterpret_cast<uint4*>(p.o + (t0 + row) * p.o_ld + (x / (D / 8)) * p.o_head + (x % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+    }
+  }
 
   int take = 0, parity = 0;
   while (cur.u < cur.u_end) {
     const PagedSpan s = cur.s;
     const int cols = s.rows * p.G;
-    // ---- the query columns: operand B of S^T, in the order of the elements that a thread loads of a key
-    uint32_t qf[NT][KSTEPS][2];
     float colf[NT][2];
     int clo[NT][2], chi[NT][2];              // keys that column 2t, 2t + 1 of the tile may see: [clo, chi)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int c = n * 8 + g;
-      const __nv_bfloat16* src = p.q + (s.row0 + c / p.G) * p.q_ld + (cur.kh * p.G + c % p.G) * p.q_head;
-#pragma unroll
-      for (int j = 0; j < C::LOADS; ++j) {
-        const int chunk = C::LOADS == 1 ? t : C::LOADS == 2 ? 2 * t + j : 2 * t + (j & 1) + 8 * (j >> 1);
-#pragma unroll
-        for (int k = 0; k < C::EPC / 4; ++k) {
-          uint2 w = make_uint2(0, 0);
-          if (c < cols) w = *reinterpret_cast<const uint2*>(src + chunk * C::EPC + 4 * k);
-          qf[n][j * (C::EPC / 4) + k][0] = w.x;
-          qf[n][j * (C::EPC / 4) + k][1] = w.y;
-        }
-      }
       float back = p.scale_log2;
       if (FP8) {
         float most = 0.f;
@@ -573,62 +599,70 @@ paged_decode_kernel(const PagedAttnParams p) {
         if (g == 0) *reinterpret_cast<float2*>(ml + (warp * COLS + n * 8 + 2 * t + h) * 2) = make_float2(M[n][h], l[n][h]);
       }
     __syncthreads();
+    // (O goes through shared memory and the workspace as the threads hold it: quad i of lane is dimensions at(i), at(i) + 1 of columns
+    // 2t, 2t + 1 of column tile i / MD)
+    float top[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int col = n * 8 + 2 * t + h;
+        top[n][h] = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PD_WARPS; ++w) top[n][h] = fmaxf(top[n][h], ml[(w * COLS + col) * 2]);
+        const float f = M[n][h] == -INFINITY ? 0.f : fast_exp2(M[n][h] - top[n][h]);
+#pragma unroll
+        for (int d = 0; d < MD; ++d) { acc[n][d][h] *= f; acc[n][d][2 + h] *= f; }
+      }
 #pragma unroll
     for (int pass = 0; pass < PD_WARPS / RB; ++pass) {
       if (warp / RB == pass) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int col = n * 8 + 2 * t + h;
-            float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < PD_WARPS; ++w) top = fmaxf(top, ml[(w * COLS + col) * 2]);
-            const float f = M[n][h] == -INFINITY ? 0.f : fast_exp2(M[n][h] - top);
-            float* dst = red_o + (warp % RB * COLS + col) * D;
-#pragma unroll
-            for (int d = 0; d < MD; ++d) {
-              const int at = C::LOADS == 4 ? 64 * (d >> 2) + 8 * g + 2 * (d & 3) : (D / 8) * g + 2 * d;
-              float2 x = make_float2(acc[n][d][h] * f, acc[n][d][2 + h] * f);
-              if (pass) {
-                const float2 y = *reinterpret_cast<const float2*>(dst + at);
-                x.x += y.x; x.y += y.y;
-              }
-              *reinterpret_cast<float2*>(dst + at) = x;
-            }
-          }
+        for (int i = 0; i < QUADS; ++i) {
+          float4* at = red_o + (warp % RB * QUADS + i) * 32 + lane;
+          const float* a = acc[i / MD][i % MD];
+          float4 x = make_float4(a[0], a[1], a[2], a[3]);
+          if (pass) { const float4 y = *at; x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w); }
+          *at = x;
+        }
       }
       __syncthreads();
     }
     const bool whole = cur.u == 0 && cur.u_end == s.units;
-    const size_t part0 = (static_cast<size_t>(blockIdx.x) * 2 + (cur.u > 0 ? 0 : 1)) * COLS;
-    for (int i = threadIdx.x; i < COLS * (D / 4); i += PD_WARPS * 32) {
-      const int col = i / (D / 4), d = (i % (D / 4)) * 4;
-      if (col >= cols) continue;
-      float top = -INFINITY, sum = 0.f;
+    const size_t part = static_cast<size_t>(blockIdx.x) * 2 + (cur.u > 0 ? 0 : 1);
+    float4* part_o = reinterpret_cast<float4*>(p.part) + part * (QUADS * 32);
+    float2* part_ml = reinterpret_cast<float2*>(p.part + static_cast<size_t>(gridDim.x) * 2 * COLS * D) + part * COLS;
 #pragma unroll
-      for (int w = 0; w < PD_WARPS; ++w) top = fmaxf(top, ml[(w * COLS + col) * 2]);
-#pragma unroll
-      for (int w = 0; w < PD_WARPS; ++w) {
-        const float2 x = *reinterpret_cast<const float2*>(ml + (w * COLS + col) * 2);
-        sum += x.x == -INFINITY ? 0.f : x.y * fast_exp2(x.x - top);
-      }
-      float4 o = *reinterpret_cast<const float4*>(red_o + col * D + d);
+    for (int i = warp; i < QUADS; i += PD_WARPS) {
+      float4 o = red_o[i * 32 + lane];
       if (RB == 2) {
-        const float4 y = *reinterpret_cast<const float4*>(red_o + ((RB - 1) * COLS + col) * D + d);
+        const float4 y = red_o[((RB - 1) * QUADS + i) * 32 + lane];
         o = make_float4(o.x + y.x, o.y + y.y, o.z + y.z, o.w + y.w);
       }
-      if (whole) {
-        // (a sum of nothing: no key, zeros; a NaN stays one)
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const long at = (s.row0 + col / p.G) * p.o_ld + (cur.kh * p.G + col % p.G) * p.o_head + d;
-        *reinterpret_cast<uint2*>(p.o + at) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
-      } else {
-        *reinterpret_cast<float4*>(p.part + (part0 + col) * D + d) = o;
-        if (d == 0) *reinterpret_cast<float2*>(p.part + static_cast<size_t>(gridDim.x) * 2 * COLS * D + (part0 + col) * 2) = make_float2(top, sum);
+      if (!whole) part_o[i * 32 + lane] = o;
+      const int n = i / MD;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int col = n * 8 + 2 * t + h;
+        float tp = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < PD_WARPS; ++w) tp = fmaxf(tp, ml[(w * COLS + col) * 2]);
+#pragma unroll
+        for (int w = 0; w < PD_WARPS; ++w) {
+          const float2 x = *reinterpret_cast<const float2*>(ml + (w * COLS + col) * 2);
+          sum += x.x == -INFINITY ? 0.f : x.y * fast_exp2(x.x - tp);
+        }
+        if (!whole) {
+          if (i % MD == 0 && g == 0) part_ml[col] = make_float2(tp, sum);
+        } else if (col < cols) {
+          // (a sum of nothing: no key, zeros; a NaN stays one)
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          const long to = (s.row0 + col / p.G) * p.o_ld + (cur.kh * p.G + col % p.G) * p.o_head + paged_dim<D, FP8>(g, i % MD);
+          *reinterpret_cast<uint32_t*>(p.o + to) = h ? pack_bf16(o.y * inv, o.w * inv) : pack_bf16(o.x * inv, o.z * inv);
+        }
       }
     }
-    if (s.extra > 0 && cur.u == 0) {
+    if (__builtin_expect(s.extra > 0 && cur.u == 0, 0)) {
       if (threadIdx.x == 0) atomicOr(p.err, 4u);
       for (long i = threadIdx.x; i < static_cast<long>(s.extra) * p.G * (D / 8); i += PD_WARPS * 32) {
         const long r = i / (p.G * (D / 8));
@@ -637,68 +671,110 @@ paged_decode_kernel(const PagedAttnParams p) {
       }
     }
     cur.next(p);
+    load_q();
   }
   cp_async_wait_all();
 }
 
-// Joins what stretches cut: block (j, column) looks at the border between stretch j and j + 1, and if it is the first one inside a
-// (sequence, kv head), adds up that one's partials in order. A warp takes every eighth of them, D / 32 dimensions a lane.
-constexpr int PJ_WARPS = 8;
-template <int D, int UNIT, int COLS>
-__global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(const PagedAttnParams p) {
-  constexpr int V = D / 32;
-  __shared__ float sum_o[PJ_WARPS][D], sum_l[PJ_WARPS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.y, ctas = p.ctas, c0 = blockIdx.x;
-  const Stretches cut(paged_total<UNIT>(p, lane), ctas);
-  const int at = cut.begin(c0 + 1);
-  int before;
-  const int b = paged_find<UNIT>(p, at, &before, lane);
-  // every block waits for the grid in front of it, so that what follows this one follows that one too
-  if (b >= p.batch.B) { asm volatile("griddepcontrol.wait;" ::: "memory"); return; }
-  const PagedSpan s = paged_span<UNIT>(p, b);
-  const int length = s.units + PD_START, kh = (at - before) / length, x = (at - before) % length, first = at - x;
-  if (x <= PD_START || cut.begin(c0) > first + PD_START || col >= s.rows * p.G) { asm volatile("griddepcontrol.wait;" ::: "memory"); return; }
-  // Its parts are the second one of stretch c0, and the first of those behind it (none of them empty: the empty ones, where there are
-  // fewer units than stretches, lie behind the end of the list).
-  int n = 1;
-  while (c0 + n < ctas && cut.begin(c0 + n) < first + length) ++n;
-  const float* ml = p.part + static_cast<size_t>(ctas) * 2 * COLS * D;
-  const auto index = [&](int i) { return (static_cast<size_t>(c0 + i) * 2 + (i == 0 ? 1 : 0)) * COLS + col; };
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  float top = -INFINITY, o[V] = {}, sum = 0.f;
-  for (int i = lane; i < n; i += 32) top = fmaxf(top, ml[index(i) * 2]);
-  top = warp_max(top);
-#pragma unroll 4
-  for (int i = warp; i < n; i += PJ_WARPS) {
-    const float2 w = *reinterpret_cast<const float2*>(ml + index(i) * 2);
-    float y[V];
-    if (V == 4) {
-      const float4 z = *reinterpret_cast<const float4*>(p.part + index(i) * D + lane * V);
-      y[0] = z.x; y[1] = z.y; y[2 % V] = z.z; y[3 % V] = z.w;
-    } else {
-      const float2 z = *reinterpret_cast<const float2*>(p.part + index(i) * D + lane * V);
-      y[0] = z.x; y[1] = z.y;
+// Joins what stretches cut: block j looks at the border between stretch j and j + 1. If it lies inside a (sequence, kv head), the blocks of
+// that one's borders share its quads of O (see above), and each adds up all the partials of its own, always in the same order. Few and
+// small blocks, so that most of them wait beside the kernel in front of them with their border looked up.
+constexpr int PJ_WARPS = 8, PJ_PARTS = 5;
+template <int D, bool FP8, int NT>
+__global__ void __launch_bounds__(PJ_WARPS * 32, 4) paged_join_kernel(const PagedAttnParams p) {
+  constexpr int COLS = 8 * NT, MD = D / 16, QUADS = NT * MD;
+  __shared__ float4 sum_o[PJ_WARPS][32], sum_ml[PJ_WARPS][4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, ctas = p.ctas;
+  asm volatile("griddepcontrol.launch_dependents;");
+  Stretches cut;
+  int at, before;
+  const int b = paged_locate<PagedDecode<D, FP8>::UNIT>(p, blockIdx.x + 1, ctas, &cut, &at, &before);
+  PagedSpan s;
+  int kh = 0, n = 0, c0 = 0;
+  if (!cut.whole && b < p.batch.B) {
+    s = paged_span<PagedDecode<D, FP8>::UNIT>(p, b);
+    const int length = cut.length(s.units);
+    kh = (at - before) / length;
+    const int x = at - before - kh * length;
+    if (x > PD_START) {
+      // Its parts are the second one of stretch c0, where its first unit lies, and the first one of each behind it up to that of its last.
+      c0 = cut.of(at - x + PD_START);
+      n = cut.of(at - x + length - 1) - c0 + 1;
     }
-    const float f = w.x == -INFINITY ? 0.f : fast_exp2(w.x - top);
-    sum += w.y * f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) o[v] += y[v] * f;
   }
+  // every block waits for the grid in front of it, so that what follows this one follows that one too
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (n == 0) return;
+  const float4* ml = reinterpret_cast<const float4*>(p.part + static_cast<size_t>(ctas) * 2 * COLS * D) + static_cast<size_t>(c0) * COLS;
+  const float4* po = reinterpret_cast<const float4*>(p.part) + static_cast<size_t>(c0) * (2 * QUADS * 32) + lane;
+  const auto index = [&](int i) { return i == 0 ? 1 : 2 * i; };
+  const int first = blockIdx.x - c0, step = n - 1, mine = (QUADS - first + step - 1) / step;   // quads first, first + step, ...
+  // Few quads: several warps on each, a part every `split`.
+  const int split = mine <= 1 ? 8 : mine <= 2 ? 4 : mine <= 4 ? 2 : 1;
+  for (int k0 = 0; k0 < mine; k0 += PJ_WARPS / split) {
+    const int k = k0 + warp / split, q = first + k * step, pair = q / MD * 4 + t;      // pair: columns 2t, 2t + 1 of the quad's tile
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    // one round of loads for up to PJ_PARTS parts, each round's maximum with the one so far
+    for (int i0 = warp % split; i0 < n && k < mine; i0 += PJ_PARTS * split) {
+      float4 y[PJ_PARTS], w[PJ_PARTS];
 #pragma unroll
-  for (int v = 0; v < V; ++v) sum_o[warp][lane * V + v] = o[v];
-  if (lane == 0) sum_l[warp] = sum;
-  __syncthreads();
-  if (threadIdx.x < D) {
-    float a = 0.f, l = 0.f;
+      for (int j = 0; j < PJ_PARTS; ++j) {
+        const int i = min(i0 + j * split, n - 1);
+        y[j] = po[(index(i) * QUADS + q) * 32];
+        w[j] = ml[index(i) * (COLS / 2) + pair];               // (m, l) of the two columns
+      }
+      float n0 = m0, n1 = m1;
 #pragma unroll
-    for (int w = 0; w < PJ_WARPS; ++w) { a += sum_o[w][threadIdx.x]; l += sum_l[w]; }
-    p.o[(s.row0 + col / p.G) * p.o_ld + (kh * p.G + col % p.G) * p.o_head + threadIdx.x] = __float2bfloat16(a * (l == 0.f ? 0.f : 1.f / l));
+      for (int j = 0; j < PJ_PARTS; ++j) {
+        if (i0 + j * split >= n) w[j].x = w[j].z = -INFINITY;
+        n0 = fmaxf(n0, w[j].x);
+        n1 = fmaxf(n1, w[j].z);
+      }
+      const float a0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - n0), a1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - n1);
+      m0 = n0; m1 = n1;
+      l0 *= a0; o.x *= a0; o.z *= a0;
+      l1 *= a1; o.y *= a1; o.w *= a1;
+#pragma unroll
+      for (int j = 0; j < PJ_PARTS; ++j) {
+        if (i0 + j * split >= n) continue;
+        const float f0 = w[j].x == -INFINITY ? 0.f : fast_exp2(w[j].x - m0), f1 = w[j].z == -INFINITY ? 0.f : fast_exp2(w[j].z - m1);
+        l0 += w[j].y * f0; o.x += y[j].x * f0; o.z += y[j].z * f0;
+        l1 += w[j].w * f1; o.y += y[j].y * f1; o.w += y[j].w * f1;
+      }
+    }
+    if (split > 1) {
+      __syncthreads();                         // (the round before has been read)
+      sum_o[warp][lane] = o;
+      if (g == 0) sum_ml[warp][t] = make_float4(m0, l0, m1, l1);
+      __syncthreads();
+      if (warp % split != 0) continue;
+      float n0 = m0, n1 = m1;
+      for (int v = 1; v < split; ++v) { n0 = fmaxf(n0, sum_ml[warp + v][t].x); n1 = fmaxf(n1, sum_ml[warp + v][t].z); }
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
+      l0 = l1 = 0.f;
+      for (int v = 0; v < split; ++v) {
+        const float4 y = sum_o[warp + v][lane], z = sum_ml[warp + v][t];
+        const float f0 = z.x == -INFINITY ? 0.f : fast_exp2(z.x - n0), f1 = z.z == -INFINITY ? 0.f : fast_exp2(z.z - n1);
+        l0 += z.y * f0; o.x += y.x * f0; o.z += y.z * f0;
+        l1 += z.w * f1; o.y += y.y * f1; o.w += y.w * f1;
+      }
+    }
+    if (k >= mine) continue;
+    const int d = paged_dim<D, FP8>(g, q % MD);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = 2 * pair + h;
+      const float l = h ? l1 : l0, inv = l == 0.f ? 0.f : 1.f / l;
+      if (c < s.rows * p.G)
+        *reinterpret_cast<uint32_t*>(p.o + (s.row0 + c / p.G) * p.o_ld + (kh * p.G + c % p.G) * p.o_head + d) =
+            h ? pack_bf16(o.y * inv, o.w * inv) : pack_bf16(o.x * inv, o.z * inv);
+    }
   }
 }
 
 template <int D, bool FP8, int NT>
 static int launch_paged_decode(PagedAttnParams& p, cudaStream_t st) {
-  using C = PagedDecode<D, FP8>;
   constexpr int smem = paged_decode_smem<D, NT>();
   static bool attr_set[64] = {false};
   int dev = 0;
@@ -707,38 +783,45 @@ static int launch_paged_decode(PagedAttnParams& p, cudaStream_t st) {
     SB_CHECK_CUDA(cudaFuncSetAttribute(paged_decode_kernel<D, FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_set[dev & 63] = true;
   }
-  paged_decode_kernel<D, FP8, NT><<<p.ctas, PD_WARPS * 32, smem, st>>>(p);
-  SB_CHECK_CUDA(cudaGetLastError());
-  if (p.ctas > 1) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.ctas - 1, min(8 * NT, p.batch.max_rows * p.G));
+  // Programmatic dependent launches: the first grid does nothing before `griddepcontrol.wait`, the second reads the batch's
+  // description before it, which was complete before the first one ran.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.ctas);
+  cfg.blockDim = dim3(PD_WARPS * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  SB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_decode_kernel<D, FP8, NT>, static_cast<const PagedAttnParams>(p)));
+  if (p.part != nullptr) {
+    cfg.gridDim = dim3(p.ctas - 1);
     cfg.blockDim = dim3(PJ_WARPS * 32);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    // programmatic dependent launch: before `griddepcontrol.wait` the grid reads the batch's description, which the kernel in
-    // front of it reads too
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    SB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<D, C::UNIT, 8 * NT>, static_cast<const PagedAttnParams>(p)));
+    cfg.dynamicSmemBytes = 0;
+    SB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<D, FP8, NT>, static_cast<const PagedAttnParams>(p)));
   }
   return SB_OK;
 }
 
-// CTAs of a call: as many as fit the GPU at a time, and no more than there can be units of work.
-static int paged_decode_ctas(int B, int Hkv, long keys, int D, bool fp8, int columns) {
+// CTAs of a call: as many as fit the GPU at a time (two to an SM), and no more than there can be places of work. *cut: whether a
+// (sequence, kv head) may be cut.
+static int paged_decode_ctas(int B, int Hkv, long keys, int D, bool fp8, bool* cut) {
   const int unit = PD_WARPS * (PD_STAGE / 2 / (fp8 ? D : 2 * D));
-  const long units = static_cast<long>(B) * Hkv * ((keys + unit - 1) / unit);
-  return static_cast<int>(min(units, static_cast<long>(columns <= 8 ? PagedShape<1>::CTAS : PagedShape<2>::CTAS) * num_sms()));
+  const long units = (keys + unit - 1) / unit;
+  const long ctas = min(static_cast<long>(B) * Hkv * (units <= PD_WHOLE ? 1 : units), 2L * num_sms());
+  *cut = units > PD_WHOLE && ctas > 1;
+  return static_cast<int>(ctas);
 }
 
 }  // namespace sb
 
-// fp32 elements of workspace that sb_paged_attention needs for `columns` = max_rows * Hq / Hkv (at most 16).
+// fp32 elements of workspace that sb_paged_attention needs for `columns` = max_rows * Hq / Hkv (at most 16); 0: none, `work` may be null.
 extern "C" long sb_paged_attention_workspace(int B, int Hkv, int P, int page, int D, int fp8, int columns) {
-  const int ctas = sb::paged_decode_ctas(B, Hkv, static_cast<long>(P) * page, D, fp8 != 0, columns);
-  return 2L * ctas * (columns <= 8 ? 8 : 16) * (D + 2);
+  bool cut;
+  const int ctas = sb::paged_decode_ctas(B, Hkv, static_cast<long>(P) * page, D, fp8 != 0, &cut);
+  return cut ? 2L * ctas * (columns <= 8 ? 8 : 16) * (D + 2) : 0;
 }
 
 // q, o bf16 `[T, Hq, D]` with strides between rows (_ld) and heads in elements; pages and their strides as in sb_paged_append. The rows
@@ -753,7 +836,7 @@ extern "C" int sb_paged_attention(const void* q, const void* kp, const void* vp,
   using namespace sb;
   const int shift = page_shift_of(page);
   SB_CHECK_ARG((D == 64 || D == 128) && shift >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && T > 0 && B > 0 && P > 0 && num_pages > 0);
-  SB_CHECK_ARG(max_rows > 0 && (starts != nullptr || (T == B && max_rows == 1)) && (ks == nullptr) == (vs == nullptr) && work != nullptr);
+  SB_CHECK_ARG(max_rows > 0 && (starts != nullptr || (T == B && max_rows == 1)) && (ks == nullptr) == (vs == nullptr));
   SB_CHECK_ARG(max_rows <= 16 && max_rows * (Hq / Hkv) <= 16);
   // places of the list of work, at the shortest unit, in 32 bits
   SB_CHECK_ARG((static_cast<double>(P) * page / 64 + 1 + PD_START) * B * Hkv < 2e9);
@@ -769,8 +852,11 @@ extern "C" int sb_paged_attention(const void* q, const void* kp, const void* vp,
   p.ks = ks; p.vs = vs; p.ks_ld = ks_ld; p.vs_ld = vs_ld;
   p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
   p.causal = causal; p.window = window; p.scale_log2 = scale * 1.4426950408889634f;
-  p.zero_tail = zero_tail; p.part = work;
-  p.ctas = paged_decode_ctas(B, Hkv, static_cast<long>(P) * page, D, fp8, max_rows * p.G);
+  p.zero_tail = zero_tail;
+  bool cut;
+  p.ctas = paged_decode_ctas(B, Hkv, static_cast<long>(P) * page, D, fp8, &cut);
+  SB_CHECK_ARG(!cut || work != nullptr);
+  p.part = cut ? work : nullptr;
   p.err = error_word();
   if (!p.err) return SB_ERR_CUDA;
   const bool two = max_rows * p.G > 8;

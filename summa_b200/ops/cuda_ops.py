@@ -653,8 +653,9 @@ def paged_attention(q, kv, rows, causal=True, window=None, scale=None, out=None)
         pages, Hkv, page, _ = k.shape
         B, P = table.shape
         most, fp8 = rows.most(T), 0 if ks is None else 1
-        ws = torch.empty(_paged_workspace(device, B, Hkv, P, page, D, fp8, most * (Hq // Hkv)), device=q.device, dtype=torch.float32)
-        N.call("sb_paged_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), N.ptr(ks), N.ptr(vs), o.data_ptr(), ws.data_ptr(),
+        need = _paged_workspace(device, B, Hkv, P, page, D, fp8, most * (Hq // Hkv))
+        ws = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
+        N.call("sb_paged_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), N.ptr(ks), N.ptr(vs), o.data_ptr(), N.ptr(ws),
                table.data_ptr(), lengths.data_ptr(), N.ptr(starts), T, B, P, Hq, Hkv, D, page, pages, most, 1 if causal else 0,
                -1 if window is None else min(int(window), 0x7fffffff), 1 if out is None else 0, 1.0 / math.sqrt(D) if scale is None else scale,
                table.stride(0), q.stride(0), q.stride(1), o.stride(0), o.stride(1), *_cache_strides(kv), N.stream())
