@@ -183,7 +183,7 @@ def paged_attention(q, kv: PagedKV, rows: PagedRows, causal=True, window=None, s
     zeros, rows behind the last sequence zeros, or as they were in `out`. Keys without a page are left out on CUDA, and set bit 4 of the
     device's error word; on the CPU they raise. A value that is not finite reaches the rows whose sequence holds it, and no others; within
     the rows of one call it may also reach those that the mask keeps from it. No gradients."""
-    paged.check_attention(q, kv, rows, window, out)
+    paged.check_attention(q, kv, rows, window, scale, out)
     _no_gradient("paged_attention", q)
     if native_enabled(q) and q.shape[2] in (64, 128):
         return _cu().paged_attention(q, kv, rows, causal, window, scale, out)

@@ -1,0 +1,670 @@
+// Attention of many query rows per sequence over the paged cache: prompt chunks behind what the cache already holds, whole prompts of
+// several sequences at once (bf16 or e4m3 pages, head_dim 64 or 128).
+//
+// The products are dense enough for the tensor cores to bound them, so they run on tcgen05 with the scores, the weights and the output
+// in tensor memory. A tile is 256 (row, head) pairs of one sequence and one kv head, rows first: pair x is row x / G, query head x % G.
+// All heads that share the kv head ride in one tile, so the keys and values that it takes from the cache, and expands, serve G times
+// the rows, and a short chunk fills the tile. Two groups of 128 pairs take turns on the tensor core:
+//   warps 0-3 / 4-7   a thread per pair: its query row to shared memory, then per block of 128 keys its scores from tensor memory,
+//                     masks, running maximum, weights back into tensor memory as operand A of the next product; at the end its output row
+//   warp 8            issues S = Q K^T
+//   warp 9            issues O += P V
+//   warps 12-15       bring keys and values from their pages into the swizzled tiles that the products read: bf16 as 16-byte
+//                     asynchronous copies, e4m3 through registers, where it becomes f16
+// (A bulk tensor copy could fetch bf16 pages, but not expand codes, nor leave out single rows of a page that hold nothing yet: what
+// lies behind a sequence's last row may be NaN, and 0 * NaN would reach its sums.) The register file is split by setmaxnreg: 512
+// threads start with 128 registers each, 65536 in all; 256 softmax threads take 192, the issuing warpgroup keeps 40 and the copying one
+// 88: 256 * 192 + 128 * 40 + 128 * 88 = 65536.
+//
+// 8 bits: as in paged_attention.cu, codes enter the products as f16, a query row scaled by a power of two to at most 2^15, the key
+// scale of each 16 keys in the factor of the scores, the value scale 2^e in the weight 2^(s + e - M) and out of it in the sum
+// l = sum w 2^-e. With bf16 pages the factor is the softmax scale and e is 0. Keys that a sequence has no page for have e = -infinity.
+//
+// With few tiles the keys are split too: each of `splits` CTAs takes a part of the tile's blocks and leaves O (unnormalised, 32
+// bits), M and l; a second kernel adds them up in order.
+#include "paged.cuh"
+
+#include <type_traits>
+
+namespace sb {
+
+struct PagedPrefillParams {
+  PagedBatch batch;
+  const __nv_bfloat16* q;
+  long q_ld, q_head;
+  __nv_bfloat16* o;
+  long o_ld, o_head;
+  const uint8_t *k, *v;
+  long k_page, k_head, v_page, v_head;     // bytes
+  const float *ks, *vs;
+  long ks_ld, vs_ld;
+  int Hq, Hkv, G;
+  int causal, window;
+  float scale_log2;
+  int zero_tail, splits, tiles;            // tiles: the most that the rows of the call can need
+  float* part;                             // [splits][tiles][Hkv]: [256][D] of O, then [256][2] of (m, l)
+  unsigned int* err;
+};
+
+constexpr int PP_THREADS = 512;
+template <int D, bool FP8>
+struct PagedPrefill {
+  static constexpr bool SEP = D == 64;                           // weights in tensor memory columns of their own
+  static constexpr int TILE = 128 * D * 2;
+  static constexpr int NSK = D == 64 ? 3 : 2, NSV = NSK;
+  static constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + NSK * TILE, OFF_SCALE = OFF_V + NSV * TILE;
+  static constexpr int RING = 8;                                 // blocks whose scales are kept: more than can be under way
+  static constexpr int OFF_BAR = OFF_SCALE + RING * 8 * 16;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+  static constexpr int COL_S = 0, COL_O = 256, COL_P = SEP ? 384 : 0, P_STRIDE = SEP ? 64 : 128;
+  static constexpr int CPR = (FP8 ? D : 2 * D) / 16;             // 16-byte chunks of a key
+  static constexpr int LOADS = 128 * CPR / 128;                  // of a copying thread, per tile of 128 keys
+  static constexpr float HEAD = FP8 ? 9.f : 0.f, SLACK = FP8 ? 6.f : 8.f;
+};
+
+// f16 operands: as make_idesc_bf16, formats 0
+__host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, int a_mn_major, int b_mn_major) {
+  return make_idesc_bf16(M, N, a_mn_major, b_mn_major) & ~((1u << 7) | (1u << 10));
+}
+
+struct PrefillTile {
+  int b, tile;                      // of sequence b
+  int row0, rows, len, hi;          // its rows of the call, tokens before, keys in the cache
+};
+
+// The tile-th tile of the call (b = B behind the last). By a whole warp.
+__device__ __forceinline__ PrefillTile prefill_tile(const PagedBatch& p, int G, int tile) {
+  const int lane = threadIdx.x & 31;
+  PrefillTile r;
+  r.b = p.B; r.tile = 0; r.row0 = r.rows = r.hi = 0; r.len = -1;
+  int front = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int rows = b0 + lane < p.B ? paged_seq(p, b0 + lane).rows : 0;
+    const int n = static_cast<int>((static_cast<long>(rows) * G + 255) / 256);
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    const unsigned in_front = __ballot_sync(0xffffffffu, front + sum <= tile);
+    if (in_front != 0xffffffffu) {
+      const int l = __popc(in_front);
+      r.b = b0 + l;
+      // tiles of a sequence from the last to the first: with a causal mask the last has the most keys, and starts first
+      const int at = tile - front - __shfl_sync(0xffffffffu, sum - n, l);
+      r.tile = __shfl_sync(0xffffffffu, n, l) - 1 - at;
+      break;
+    }
+    front += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (r.b < p.B) {
+    const PagedSeq s = paged_seq(p, r.b);
+    r.row0 = s.row0; r.rows = s.rows; r.len = s.len;
+    const long cap = min(static_cast<long>(p.P) << p.page_shift, 0x7fffff00L);
+    r.hi = s.len < 0 ? 0 : static_cast<int>(min(static_cast<long>(s.len) + s.rows, cap));
+  }
+  return r;
+}
+
+template <int D, bool FP8>
+__global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const PagedPrefillParams p) {
+  using C = PagedPrefill<D, FP8>;
+  constexpr int NSK = C::NSK, NSV = C::NSV;
+  extern __shared__ uint8_t smem_raw[];
+  asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* q_full = bars + 0;    // 256 arrivals
+  uint64_t* s_full = bars + 1;    // [2]
+  uint64_t* s_free = bars + 3;    // [2], 128 arrivals: the group has read S (SEP only)
+  uint64_t* p_full = bars + 5;    // [2], 128 arrivals
+  uint64_t* o_full = bars + 7;    // [2] the product of a block is complete
+  uint64_t* k_full = bars + 9;    // [NSK], 128 arrivals
+  uint64_t* k_empty = bars + 12;
+  uint64_t* v_full = bars + 15;   // [NSV], 128 arrivals
+  uint64_t* v_empty = bars + 18;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float4* scales = reinterpret_cast<float4*>(smem + C::OFF_SCALE);       // [RING][8]: key factor, e, 2^-e
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int kh = blockIdx.x;
+  const PrefillTile tl = prefill_tile(p.batch, p.G, blockIdx.y);
+  if (p.zero_tail) {
+    const int t0 = paged_tail(p.batch);
+    const long n = static_cast<long>(p.batch.T - t0) * p.Hq * (D / 8);
+    const long cta = blockIdx.x + static_cast<long>(gridDim.x) * (blockIdx.y + static_cast<long>(gridDim.y) * blockIdx.z);
+    const long ctas = static_cast<long>(gridDim.x) * gridDim.y * gridDim.z;
+    for (long i = cta * PP_THREADS + threadIdx.x; i < n; i += ctas * PP_THREADS) {
+      const long row = i / (p.Hq * (D / 8));
+      const int x = static_cast<int>(i % (p.Hq * (D / 8)));
+      *reinterpret_cast<uint4*>(p.o + (t0 + row) * p.o_ld + (x / (D / 8)) * p.o_head + (x % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  if (tl.b >= p.batch.B) return;
+
+  // the tile's pairs and the keys that any of them sees
+  const long pairs = static_cast<long>(tl.rows) * p.G, x0 = static_cast<long>(tl.tile) * 256;
+  const int tiles_here = pairs - x0 > 128 ? 2 : 1;               // groups that have pairs
+  const int first_row = static_cast<int>(x0 / p.G), last_row = static_cast<int>((min(pairs, x0 + 256) - 1) / p.G);
+  int lo = 0, hi = tl.hi;
+  if (tl.len >= 0) {
+    if (p.causal) hi = static_cast<int>(min(static_cast<long>(hi), static_cast<long>(tl.len) + last_row + 1));
+    else if (p.window >= 0) hi = static_cast<int>(min(static_cast<long>(hi), static_cast<long>(tl.len) + last_row + p.window + 1));
+    if (p.window >= 0) lo = static_cast<int>(max(static_cast<long>(tl.len) + first_row - p.window, 0L));
+  }
+  int j0 = lo / 128, j1 = (hi + 127) / 128;
+  if (hi <= lo) j1 = j0;
+  if (p.splits > 1) {
+    const int per = (j1 - j0 + p.splits - 1) / p.splits, end = j1;
+    j0 = min(j0 + static_cast<int>(blockIdx.z) * per, end);
+    j1 = min(j0 + per, end);
+  }
+  const int nblk = j1 - j0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 256);
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&s_full[a], 1); mbar_init(&s_free[a], 128); mbar_init(&p_full[a], 128); mbar_init(&o_full[a], 1);
+    }
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(&k_full[s], 128); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 128); mbar_init(&v_empty[s], 1);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp >= 12) {
+    // ---------------------------------------------------------------- copies
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    const int tid = threadIdx.x - 384, shift = p.batch.page_shift, mask = (1 << shift) - 1;
+    const int* table = p.batch.table + tl.b * p.batch.table_ld;
+    const uint8_t *kb = p.k + kh * p.k_head, *vb = p.v + kh * p.v_head;
+    // chunk i of a thread: row r(i), chunk c of the row; 16 keys of one page share a look-up
+    constexpr int RPI = 128 / C::CPR, IDS = RPI >= 16 ? C::LOADS : 8;     // rows of a step, pages that a thread meets in a tile
+    const int r0 = tid / C::CPR, c = tid % C::CPR;
+    auto row_of = [&](int i) { return i * RPI + r0; };
+    int id[IDS] = {}, next[IDS];
+    auto look_up = [&](int j, int* to) {
+#pragma unroll
+      for (int i = 0; i < IDS; ++i) {
+        const int key = j * 128 + (RPI >= 16 ? row_of(i) : i * 16);
+        to[i] = -2;
+        if (j < j1 && (key | 15) >= lo && (key & ~15) < hi) to[i] = table[key >> shift];
+      }
+    };
+    auto source = [&](const uint8_t* base, long stride, int i, int j, bool* in) -> const uint8_t* {
+      const int page = id[RPI >= 16 ? i : i * RPI / 16], key = j * 128 + row_of(i);
+      *in = static_cast<unsigned>(page) < static_cast<unsigned>(p.batch.num_pages) && key >= lo && key < hi;
+      return base + (*in ? static_cast<uint64_t>(page) * static_cast<uint32_t>(stride) + static_cast<uint32_t>((key & mask) * (C::CPR * 16) + c * 16) : 0);
+    };
+    // where 8 elements (16 bytes) of row r, elements 8 e .. lie in a tile: 64 elements a row of a swizzled half
+    auto place = [&](int r, int e) -> uint32_t { return (e >> 3) * 16384 + r * 128 + (((e & 7) ^ (r & 7)) << 4); };
+    bool ok = true;
+    uint4 raw[FP8 ? C::LOADS : 1];
+    look_up(j0, next);
+    for (int n = 0; n < 2 * nblk && ok; ++n) {                   // K and V of block 0, of block 1, ...
+      const int i = n >> 1, j = j0 + i;
+      const bool is_v = n & 1;
+      if (!is_v) {
+#pragma unroll
+        for (int x = 0; x < IDS; ++x) id[x] = next[x];
+        look_up(j + 1, next);
+        // the scales of its groups of 16 keys, read by the softmax threads behind S
+        if (tid < 8) {
+          const int key = j * 128 + tid * 16;
+          int page = -1;
+          if (key + 16 > lo && key < hi) {
+            page = table[key >> shift];
+            if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.batch.num_pages)) { page = -1; atomicOr(p.err, 4u); }
+          }
+          float4 f = make_float4(1.f, page >= 0 ? 0.f : -INFINITY, page >= 0 ? 1.f : 0.f, 0.f);
+          if (FP8 && page >= 0) {
+            const int e = min(max(scale_exp(p.vs[page * p.vs_ld + kh]), PAGED_LEAST_EXP), PAGED_MOST_EXP);
+            f = make_float4(p.ks[page * p.ks_ld + kh], static_cast<float>(e), exp_scale(-e), 0.f);
+          }
+          scales[(i % C::RING) * 8 + tid] = f;
+        }
+      }
+      const int s = i % (is_v ? NSV : NSK);
+      uint8_t* dst = smem + (is_v ? C::OFF_V : C::OFF_K) + s * C::TILE;
+      const uint8_t* base = is_v ? vb : kb;
+      const long stride = is_v ? p.v_page : p.k_page;
+      if (FP8) {
+#pragma unroll
+        for (int x = 0; x < C::LOADS; ++x) {
+          bool in;
+          const uint8_t* src = source(base, stride, x, j, &in);
+          raw[x] = make_uint4(0, 0, 0, 0);
+          if (in) raw[x] = *reinterpret_cast<const uint4*>(src);
+        }
+      }
+      ok = mbar_wait(is_v ? &v_empty[s] : &k_empty[s], ((i / (is_v ? NSV : NSK)) & 1) ^ 1, abort_flag, p.err);
+      if (!ok) break;
+      if (FP8) {
+#pragma unroll
+        for (int x = 0; x < C::LOADS; ++x) {
+          const uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+          uint32_t h[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+                : "=r"(h[2 * k]), "=r"(h[2 * k + 1]) : "r"(w[k]));
+          const int r = row_of(x);
+          *reinterpret_cast<uint4*>(dst + place(r, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(dst + place(r, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(is_v ? &v_full[s] : &k_full[s]);
+      } else {
+#pragma unroll
+        for (int x = 0; x < C::LOADS; ++x) {
+          bool in;
+          const uint8_t* src = source(base, stride, x, j, &in);
+          cp_async16_zfill(smem_u32(dst + place(row_of(x), c)), src, in ? 16 : 0);
+        }
+        cp_async_commit();
+        // the tile before this one has landed: hand it over
+        if (n > 0) {
+          cp_async_wait_group<1>();
+          fence_proxy_async_smem();
+          const int i1 = (n - 1) >> 1;
+          mbar_arrive(is_v ? &k_full[i1 % NSK] : &v_full[i1 % NSV]);
+        }
+      }
+    }
+    if (!FP8) {
+      cp_async_wait_group<0>();
+      if (ok && nblk > 0) {
+        fence_proxy_async_smem();
+        mbar_arrive(&v_full[(nblk - 1) % NSV]);
+      }
+    }
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 8 && lane == 0 && nblk > 0) {
+      // -------------------------------------------------------------- S = Q K^T
+      constexpr uint32_t idesc = FP8 ? make_idesc_f16(128, 128, 0, 0) : make_idesc_bf16(128, 128, 0, 0);
+      const uint32_t q_base = smem_u32(smem), k_base = smem_u32(smem + C::OFF_K);
+      bool ok = mbar_wait(q_full, 0, abort_flag, p.err);
+      for (int i = 0; i < nblk && ok; ++i) {
+        const int ks = i % NSK;
+        if (!mbar_wait(&k_full[ks], (i / NSK) & 1, abort_flag, p.err)) break;
+        for (int a = 0; a < tiles_here && ok; ++a) {
+          if (i > 0) {
+            ok = C::SEP ? mbar_wait(&s_free[a], (i - 1) & 1, abort_flag, p.err) : mbar_wait(&o_full[a], (i - 1) & 1, abort_flag, p.err);
+            if (!ok) break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
+            umma_bf16(tmem_base + C::COL_S + a * 128, make_smem_desc_sw128(q_base + a * C::TILE + off, 16, 1024),
+                      make_smem_desc_sw128(k_base + ks * C::TILE + off, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[a]);
+        }
+        if (ok) umma_commit(&k_empty[ks]);
+      }
+    } else if (warp == 9 && lane == 0 && nblk > 0) {
+      // -------------------------------------------------------------- O += P V
+      constexpr uint32_t idesc = FP8 ? make_idesc_f16(128, D, 0, 1) : make_idesc_bf16(128, D, 0, 1);
+      const uint32_t v_base = smem_u32(smem + C::OFF_V);
+      bool ok = true;
+      for (int i = 0; i < nblk && ok; ++i) {
+        const int vs = i % NSV;
+        if (!mbar_wait(&v_full[vs], (i / NSV) & 1, abort_flag, p.err)) break;
+        for (int a = 0; a < tiles_here && ok; ++a) {
+          if (!mbar_wait(&p_full[a], i & 1, abort_flag, p.err)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            umma_bf16_ta(tmem_base + C::COL_O + a * D, tmem_base + C::COL_P + a * C::P_STRIDE + 8 * kk,
+                         make_smem_desc_sw128(v_base + vs * C::TILE + kk * 2048, 16384, 1024), idesc, (i > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&o_full[a]);
+        }
+        if (ok) umma_commit(&v_empty[vs]);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- softmax, a thread per pair
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    const int a = warp >> 2, t = threadIdx.x & 127;
+    const long x = x0 + a * 128 + t;
+    const bool live = x < pairs;
+    const int row = live ? static_cast<int>(x / p.G) : 0, head = kh * p.G + (live ? static_cast<int>(x % p.G) : 0);
+    const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem_base + C::COL_S + a * 128 + lane_sel;
+    const uint32_t t_o = tmem_base + C::COL_O + a * D + lane_sel;
+    const uint32_t t_p = tmem_base + C::COL_P + a * C::P_STRIDE + lane_sel;
+
+    // the query row into its tile; in 8 bits as f16, scaled by a power of two
+    float back = p.scale_log2;
+    {
+      uint4 w[D / 8];
+      const __nv_bfloat16* src = p.q + (tl.row0 + row) * p.q_ld + head * p.q_head;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        w[i] = make_uint4(0, 0, 0, 0);
+        if (live) w[i] = *reinterpret_cast<const uint4*>(src + i * 8);
+      }
+      if (FP8) {
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) most = fmaxf(most, fmaxf(fabsf(bf16_lo(u[k])), fabsf(bf16_hi(u[k]))));
+        }
+        int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100);
+        if (most == 0.f || !(most < INFINITY)) e = 14;
+        const float mul = exp_scale(14 - e);
+        back *= exp_scale(e - 14);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const __half2 h = __floats2half2_rn(bf16_lo(u[k]) * mul, bf16_hi(u[k]) * mul);
+            u[k] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          w[i] = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+      }
+      uint8_t* tile = smem + a * C::TILE;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(tile + (i >> 3) * 16384 + t * 128 + (((i & 7) ^ (t & 7)) << 4)) = w[i];
+      fence_proxy_async_smem();
+      mbar_arrive(q_full);
+    }
+
+    // keys that this pair sees: [klo, khi)
+    const long pos = static_cast<long>(tl.len) + row;
+    int klo = 0, khi = tl.hi;
+    if (p.causal) khi = static_cast<int>(min(static_cast<long>(khi), pos + 1));
+    if (p.window >= 0) {
+      klo = static_cast<int>(max(pos - p.window, 0L));
+      khi = static_cast<int>(min(static_cast<long>(khi), pos + p.window + 1));
+    }
+    if (!live) khi = 0;
+    float m_ref = -INFINITY, l = 0.f;
+    bool ok = a < tiles_here;
+    const bool group = ok;
+    for (int i = 0; i < nblk && ok; ++i) {
+      const int kv0 = (j0 + i) * 128;
+      if (!mbar_wait(&s_full[a], i & 1, abort_flag, p.err)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t v[128];
+      tmem_ld_32x32b_x32(t_s, v);
+      tmem_ld_32x32b_x32(t_s + 32, v + 32);
+      tmem_ld_32x32b_x32(t_s + 64, v + 64);
+      tmem_ld_32x32b_x32(t_s + 96, v + 96);
+      tmem_ld_wait();
+      if (C::SEP) {
+        tc_fence_before();
+        mbar_arrive(&s_free[a]);
+      }
+      const float4* sc = scales + (i % C::RING) * 8;
+      bool masked = kv0 < klo || kv0 + 128 > khi;
+      if (masked) {
+        const int from = klo - kv0, to = khi - kv0;
+#pragma unroll
+        for (int k = 0; k < 128; ++k) v[k] = (k >= from && k < to) ? v[k] : 0xff800000u;   // -inf
+      }
+      float m_blk = -INFINITY;
+#pragma unroll
+      for (int gp = 0; gp < 8; ++gp) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(v[gp * 16 + k]), __uint_as_float(v[gp * 16 + k + 1])));
+        const float4 f = sc[gp];
+        m_blk = fmaxf(m_blk, fmaf(mx, fmaxf(back * f.x, 1e-37f), f.y));
+        masked |= f.z == 0.f;
+      }
+      const bool grow = m_blk > m_ref + C::SLACK;
+      if (i > 0 && !mbar_wait(&o_full[a], (i - 1) & 1, abort_flag, p.err)) { ok = false; break; }
+      tc_fence_after();
+      if (__any_sync(0xffffffffu, grow)) {
+        const float m_new = grow ? m_blk : m_ref;
+        const float alpha = (m_ref == -INFINITY) ? 0.f : fast_exp2(m_ref - m_new);
+        if (i > 0) {
+#pragma unroll
+          for (int cc = 0; cc < D / 16; ++cc) {
+            uint32_t o16[16];
+            tmem_ld_32x32b_x16(t_o + cc * 16, o16);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o16[k] = __float_as_uint(__uint_as_float(o16[k]) * (grow ? alpha : 1.f));
+            tmem_st_32x32b_x16(t_o + cc * 16, o16);
+          }
+        }
+        if (grow) { l *= alpha; m_ref = m_new; }
+      }
+      const float nm = C::HEAD - (m_ref == -INFINITY ? 0.f : m_ref);
+      // (the FMA form of the exponential makes 2^-126 of -infinity: where there are masked keys, which have to weigh nothing even beside
+      // a sum of next to nothing, it is left out)
+      auto weights = [&](auto poly) {
+        constexpr bool POLY = decltype(poly)::value;
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            const float4 f = sc[cc * 2 + hh];
+            const float fs = fmaxf(back * f.x, 1e-37f);
+            const uint64_t f2 = f2_pack(fs, fs), n2 = f2_pack(f.y + nm, f.y + nm);
+            uint64_t sum2 = f2_pack(0.f, 0.f);
+#pragma unroll
+            for (int jj = 0; jj < 8; ++jj) {
+              const int k = cc * 32 + hh * 16 + 2 * jj;
+              float y0, y1, e0, e1;
+              f2_unpack(f2_fma(f2_pack_u(v[k], v[k + 1]), f2, n2), y0, y1);
+              // one pair of four on the FMA pipe, as in attention_fwd.cu
+              if (POLY && jj % 4 == 3) exp2_poly2(y0, y1, e0, e1);
+              else { e0 = fast_exp2(y0); e1 = fast_exp2(y1); }
+              sum2 = f2_add(sum2, f2_pack(e0, e1));
+              if (FP8) {
+                const __half2 h = __floats2half2_rn(e0, e1);
+                pk[hh * 8 + jj] = *reinterpret_cast<const uint32_t*>(&h);
+              } else {
+                pk[hh * 8 + jj] = pack_bf16(e0, e1);
+              }
+            }
+            float s0, s1;
+            f2_unpack(sum2, s0, s1);
+            l = FP8 ? fmaf(s0 + s1, f.z, l) : l + (s0 + s1);
+          }
+          tmem_st_32x32b_x16(t_p + cc * 16, pk);
+        }
+      };
+      if (__any_sync(0xffffffffu, masked)) weights(std::false_type{});
+      else weights(std::true_type{});
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[a]);
+    }
+    const bool have = group && ok && nblk > 0 && mbar_wait(&o_full[a], (nblk - 1) & 1, abort_flag, p.err);
+    if (have) tc_fence_after();
+    if (p.splits > 1) {
+      const size_t at = ((static_cast<size_t>(blockIdx.z) * p.tiles + blockIdx.y) * p.Hkv + kh) * 256 + a * 128 + t;
+      float* po = p.part + at * D;
+      float* ml = p.part + static_cast<size_t>(p.splits) * p.tiles * p.Hkv * 256 * D + at * 2;
+#pragma unroll
+      for (int cc = 0; cc < D / 16; ++cc) {
+        uint32_t o16[16];
+        if (have) {
+          tmem_ld_32x32b_x16(t_o + cc * 16, o16);
+          tmem_ld_wait();
+        }
+        if (live && have) {
+#pragma unroll
+          for (int k = 0; k < 16; k += 4)
+            *reinterpret_cast<uint4*>(po + cc * 16 + k) = make_uint4(o16[k], o16[k + 1], o16[k + 2], o16[k + 3]);
+        }
+      }
+      if (live) *reinterpret_cast<float2*>(ml) = make_float2(have ? m_ref : -INFINITY, l);
+    } else {
+      // (a sum of nothing: no key, zeros; a NaN stays one)
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      __nv_bfloat16* dst = p.o + (tl.row0 + row) * p.o_ld + head * p.o_head;
+#pragma unroll
+      for (int cc = 0; cc < D / 16; ++cc) {
+        uint32_t o16[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o16[k] = 0u;
+        if (have) {
+          tmem_ld_32x32b_x16(t_o + cc * 16, o16);
+          tmem_ld_wait();
+        }
+        if (live) {
+#pragma unroll
+          for (int k = 0; k < 16; k += 8) {
+            uint4 w;
+            w.x = pack_bf16(__uint_as_float(o16[k + 0]) * inv, __uint_as_float(o16[k + 1]) * inv);
+            w.y = pack_bf16(__uint_as_float(o16[k + 2]) * inv, __uint_as_float(o16[k + 3]) * inv);
+            w.z = pack_bf16(__uint_as_float(o16[k + 4]) * inv, __uint_as_float(o16[k + 5]) * inv);
+            w.w = pack_bf16(__uint_as_float(o16[k + 6]) * inv, __uint_as_float(o16[k + 7]) * inv);
+            *reinterpret_cast<uint4*>(dst + cc * 16 + k) = w;
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Adds up the parts of a tile: block (kv head, tile), a warp per pair, D / 32 dimensions a lane.
+template <int D>
+__global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PagedPrefillParams p) {
+  constexpr int V = D / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kh = blockIdx.x;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const PrefillTile tl = prefill_tile(p.batch, p.G, blockIdx.y);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (tl.b >= p.batch.B) return;
+  const long pairs = static_cast<long>(tl.rows) * p.G, x0 = static_cast<long>(tl.tile) * 256;
+  const size_t stride = static_cast<size_t>(p.tiles) * p.Hkv * 256;                 // pairs between two splits
+  const float* ml0 = p.part + p.splits * stride * D;
+  for (int r = blockIdx.z * 8 + warp; r < 256 && x0 + r < pairs; r += 8 * gridDim.z) {
+    const size_t at = (static_cast<size_t>(blockIdx.y) * p.Hkv + kh) * 256 + r;
+    float top = -INFINITY, sum = 0.f, o[V] = {};
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml0[(s * stride + at) * 2]);
+    for (int s = 0; s < p.splits; ++s) {
+      const float2 w = *reinterpret_cast<const float2*>(ml0 + (s * stride + at) * 2);
+      if (w.x == -INFINITY && w.y == 0.f) continue;      // no key there: its O was not written
+      const float f = w.x == -INFINITY ? 0.f : fast_exp2(w.x - top);
+      sum += w.y * f;
+      const float* y = p.part + (s * stride + at) * D + lane * V;
+      if (V == 4) {
+        const float4 z = *reinterpret_cast<const float4*>(y);
+        o[0] += z.x * f; o[1] += z.y * f; o[2 % V] += z.z * f; o[3 % V] += z.w * f;
+      } else {
+        const float2 z = *reinterpret_cast<const float2*>(y);
+        o[0] += z.x * f; o[1] += z.y * f;
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    __nv_bfloat16* dst = p.o + (tl.row0 + (x0 + r) / p.G) * p.o_ld + (kh * p.G + (x0 + r) % p.G) * p.o_head + lane * V;
+    if (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2 % V] * inv, o[3 % V] * inv));
+    else *reinterpret_cast<uint32_t*>(dst) = pack_bf16(o[0] * inv, o[1] * inv);
+  }
+}
+
+template <int D, bool FP8>
+static int launch_paged_prefill(PagedPrefillParams& p, cudaStream_t st) {
+  using C = PagedPrefill<D, FP8>;
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  SB_CHECK_CUDA(cudaGetDevice(&dev));
+  if (!attr_set[dev & 63]) {
+    SB_CHECK_CUDA(cudaFuncSetAttribute(paged_prefill_kernel<D, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    attr_set[dev & 63] = true;
+  }
+  // Programmatic dependent launches: the first grid does nothing before `griddepcontrol.wait`, the second reads the batch's
+  // description before it, which was complete before the first one let it start.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.Hkv, p.tiles, p.splits);
+  cfg.blockDim = dim3(PP_THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  SB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_prefill_kernel<D, FP8>, static_cast<const PagedPrefillParams>(p)));
+  if (p.splits > 1) {
+    cfg.gridDim = dim3(p.Hkv, p.tiles, 4);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    SB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_prefill_join_kernel<D>, static_cast<const PagedPrefillParams>(p)));
+  }
+  return SB_OK;
+}
+
+// Tiles that T rows of B sequences can need, and parts that the keys of a tile are split into: as many as make the rounds of CTAs over
+// the GPU the shortest, a part costing two blocks of keys beside its own (a start, and its share of the join).
+static int paged_prefill_shape(int T, int B, int Hkv, int G, long keys, int* splits) {
+  const long tiles = static_cast<long>(T) * G / 256 + min(B, T);
+  const long items = tiles * Hkv, blocks = (keys + 127) / 128, sms = num_sms();
+  long best = 0;
+  *splits = 1;
+  for (int s = 1; s <= 16 && s <= blocks; ++s) {
+    const long cost = (items * s + sms - 1) / sms * ((blocks + s - 1) / s + (s > 1 ? 2 : 0));
+    if (s == 1 || cost < best) { best = cost; *splits = s; }
+  }
+  return static_cast<int>(tiles);
+}
+
+}  // namespace sb
+
+// fp32 elements of workspace that sb_paged_prefill needs; 0: none, `work` may be null.
+extern "C" long sb_paged_prefill_workspace(int T, int B, int Hkv, int G, int P, int page, int D) {
+  int splits;
+  const long tiles = sb::paged_prefill_shape(T, B, Hkv, G, static_cast<long>(P) * page, &splits);
+  return splits > 1 ? splits * tiles * Hkv * 256L * (D + 2) : 0;
+}
+
+// As sb_paged_attention, for any number of rows per sequence and of query heads per kv head.
+extern "C" int sb_paged_prefill(const void* q, const void* kp, const void* vp, const float* ks, const float* vs, void* o, float* work,
+                                const int* table, const int* lengths, const int* starts, int T, int B, int P, int Hq, int Hkv, int D,
+                                int page, int num_pages, int causal, int window, int zero_tail, float scale, long table_ld, long q_ld,
+                                long q_head, long o_ld, long o_head, long k_page, long k_head, long v_page, long v_head, long ks_ld,
+                                long vs_ld, cudaStream_t st) {
+  using namespace sb;
+  const int shift = page_shift_of(page);
+  SB_CHECK_ARG((D == 64 || D == 128) && shift >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && T > 0 && B > 0 && P > 0 && num_pages > 0);
+  SB_CHECK_ARG((starts != nullptr || T == B) && (ks == nullptr) == (vs == nullptr) && scale > 0.f);
+  const bool fp8 = ks != nullptr;
+  const long size = fp8 ? 1 : 2;
+  SB_CHECK_ARG(k_page >= 0 && v_page >= 0 && k_head >= 0 && v_head >= 0 && k_page * size < (1L << 32) && v_page * size < (1L << 32));
+  PagedPrefillParams p;
+  p.batch = PagedBatch{table, lengths, starts, table_ld, P, B, T, T, shift, num_pages};
+  p.q = static_cast<const __nv_bfloat16*>(q); p.q_ld = q_ld; p.q_head = q_head;
+  p.o = static_cast<__nv_bfloat16*>(o); p.o_ld = o_ld; p.o_head = o_head;
+  p.k = static_cast<const uint8_t*>(kp); p.v = static_cast<const uint8_t*>(vp);
+  p.k_page = k_page * size; p.k_head = k_head * size; p.v_page = v_page * size; p.v_head = v_head * size;
+  p.ks = ks; p.vs = vs; p.ks_ld = ks_ld; p.vs_ld = vs_ld;
+  p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
+  p.causal = causal; p.window = window; p.scale_log2 = scale * 1.4426950408889634f;
+  p.zero_tail = zero_tail; p.part = work;
+  p.tiles = paged_prefill_shape(T, B, Hkv, p.G, static_cast<long>(P) * page, &p.splits);
+  SB_CHECK_ARG(p.tiles <= 65535 && (p.splits == 1 || work != nullptr));
+  p.err = error_word();
+  if (!p.err) return SB_ERR_CUDA;
+  if (D == 64) return fp8 ? launch_paged_prefill<64, true>(p, st) : launch_paged_prefill<64, false>(p, st);
+  return fp8 ? launch_paged_prefill<128, true>(p, st) : launch_paged_prefill<128, false>(p, st);
+}

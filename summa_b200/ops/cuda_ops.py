@@ -630,9 +630,14 @@ def _gains(g: torch.Tensor) -> torch.Tensor:
     return g.clone() if g.data_ptr() % 16 else g
 
 
+N.register("sb_paged_prefill", [N.P] * 10 + [N.I] * 11 + [N.F] + [N.L] * 11 + [N.P])
+N.register("sb_paged_prefill_workspace", [N.I] * 7, restype=ctypes.c_long)
+PAGED_COLUMNS = 16      # rows of a sequence times query heads of a kv head that the streaming kernel takes; beyond, the tiled one
+
+
 @functools.lru_cache(maxsize=256)
-def _paged_workspace(device, B, Hkv, P, page, D, fp8, columns):
-    return N.call_value("sb_paged_attention_workspace", B, Hkv, P, page, D, fp8, columns)
+def _paged_workspace(device, name, *sizes):
+    return N.call_value(name, *sizes)
 
 
 def paged_attention(q, kv, rows, causal=True, window=None, scale=None, out=None):
@@ -652,11 +657,16 @@ def paged_attention(q, kv, rows, causal=True, window=None, scale=None, out=None)
         table, lengths, starts, _ = rows
         pages, Hkv, page, _ = k.shape
         B, P = table.shape
-        most, fp8 = rows.most(T), 0 if ks is None else 1
-        need = _paged_workspace(device, B, Hkv, P, page, D, fp8, most * (Hq // Hkv))
+        most, G = rows.most(T), Hq // Hkv
+        if most * G <= PAGED_COLUMNS:
+            name, most = "sb_paged_attention", (most,)
+            need = _paged_workspace(device, "sb_paged_attention_workspace", B, Hkv, P, page, D, 0 if ks is None else 1, most[0] * G)
+        else:
+            name, most = "sb_paged_prefill", ()
+            need = _paged_workspace(device, "sb_paged_prefill_workspace", T, B, Hkv, G, P, page, D)
         ws = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
-        N.call("sb_paged_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), N.ptr(ks), N.ptr(vs), o.data_ptr(), N.ptr(ws),
-               table.data_ptr(), lengths.data_ptr(), N.ptr(starts), T, B, P, Hq, Hkv, D, page, pages, most, 1 if causal else 0,
+        N.call(name, q.data_ptr(), k.data_ptr(), v.data_ptr(), N.ptr(ks), N.ptr(vs), o.data_ptr(), N.ptr(ws),
+               table.data_ptr(), lengths.data_ptr(), N.ptr(starts), T, B, P, Hq, Hkv, D, page, pages, *most, 1 if causal else 0,
                -1 if window is None else min(int(window), 0x7fffffff), 1 if out is None else 0, 1.0 / math.sqrt(D) if scale is None else scale,
                table.stride(0), q.stride(0), q.stride(1), o.stride(0), o.stride(1), *_cache_strides(kv), N.stream())
     if out is not None and o is not out:

@@ -102,7 +102,7 @@ def check_append(qkv, q_gamma, k_gamma, cos, sin, Hq, Hkv, D, kv, rows, out) -> 
     check(qkv, Hkv, D, kv, rows)
 
 
-def check_attention(q, kv, rows, window, out) -> None:
+def check_attention(q, kv, rows, window, scale, out) -> None:
     if q.dim() != 3 or kv.k.dim() != 4:
         raise ValueError("q: [T, Hq, D]; pages: [num_pages, Hkv, page, D]")
     Hq, Hkv = q.shape[1], kv.k.shape[1]
@@ -110,6 +110,8 @@ def check_attention(q, kv, rows, window, out) -> None:
         raise ValueError(f"{Hq} query heads over {Hkv} kv heads")
     if window is not None and window < 0:
         raise ValueError(f"window {window}")
+    if scale is not None and not 0.0 < scale < math.inf:
+        raise ValueError(f"scale {scale}: it has to be positive")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device):
         raise ValueError(f"out: {list(q.shape)} of the type and device of the rows")
     check(q, Hkv, q.shape[2], kv, rows)
