@@ -21,8 +21,8 @@
 //
 // 8 bits: e4m3 becomes f16 exactly. A query column is scaled by a power of two to at most 2^14 (f16 then holds every element down
 // to 2^-28 of the largest exactly), the scores come back with that, the scale of the page and the softmax scale in one factor.
-// The values' scale 2^e goes into the weight, w = 2^(s + e - M) with M the running maximum of s + e, and out of it in the sum of
-// weights, l = sum w 2^-e, in 32 bits: so w is at most 1 whatever the pages' scales (2^4 with a
+// The values' scale 2^e goes into the weight, w = 2^(s + e - M) with M the running maximum of s + e, beside a sum l of 2^(s - M) in 32
+// bits: so w is at most 1 whatever the pages' scales (2^4 with a
 // reference that only moves when a score passes it by that), and goes into the product as w 2^11, where f16 has 25 binary orders of
 // full precision below 1 and ten more of less. bf16 pages: w = 2^(s - M) in bf16, as the rows of a bf16 product must be.
 #include "paged.cuh"
@@ -464,24 +464,23 @@ paged_decode_kernel(const PagedAttnParams p) {
         }
       }
       // ---- scores with their scales and masks; in 8 bits they are s + e from here on, e the value scale's exponent
-      float vinv[MT];
+      float ve[MT];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        float kscale = 1.f, ve = 0.f;
-        vinv[m] = 1.f;
+        float kscale = 1.f;
+        ve[m] = 0.f;
         if (FP8) {
           kscale = *reinterpret_cast<const float*>(mt_meta + m * 4);
           const int e = min(max(scale_exp(*reinterpret_cast<const float*>(mt_meta + 16 + m * 4)), PAGED_LEAST_EXP), PAGED_MOST_EXP);
-          ve = static_cast<float>(e);
-          vinv[m] = exp_scale(-e);
+          ve[m] = static_cast<float>(e);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float f = FP8 ? colf[n][h] * kscale : colf[n][h];
-            sc[n][m][h] = FP8 ? fmaf(sc[n][m][h], f, ve) : sc[n][m][h] * f;
-            sc[n][m][2 + h] = FP8 ? fmaf(sc[n][m][2 + h], f, ve) : sc[n][m][2 + h] * f;
+            sc[n][m][h] = FP8 ? fmaf(sc[n][m][h], f, ve[m]) : sc[n][m][h] * f;
+            sc[n][m][2 + h] = FP8 ? fmaf(sc[n][m][2 + h], f, ve[m]) : sc[n][m][2 + h] * f;
           }
         }
       }
@@ -537,8 +536,10 @@ paged_decode_kernel(const PagedAttnParams p) {
         for (int m = 0; m < MT; ++m) {
           const float w0 = fast_exp2(sc[n][m][0] - r0), w1 = fast_exp2(sc[n][m][1] - r1);
           const float w2 = fast_exp2(sc[n][m][2] - r0), w3 = fast_exp2(sc[n][m][3] - r1);
-          l[n][0] = FP8 ? fmaf(w0 + w2, vinv[m], l[n][0]) : l[n][0] + (w0 + w2);
-          l[n][1] = FP8 ? fmaf(w1 + w3, vinv[m], l[n][1]) : l[n][1] + (w1 + w3);
+          // (from the scores, not as w 2^-e: of pages 2^120 apart the one's w is nothing beside the other's, its share of l is not)
+          const float q0 = r0 + ve[m], q1 = r1 + ve[m];
+          l[n][0] += FP8 ? fast_exp2(sc[n][m][0] - q0) + fast_exp2(sc[n][m][2] - q0) : w0 + w2;
+          l[n][1] += FP8 ? fast_exp2(sc[n][m][1] - q1) + fast_exp2(sc[n][m][3] - q1) : w1 + w3;
           pf[n][m][0] = transpose8x8(FP8 ? pack_f16(w0, w1) : pack_bf16(w0, w1));
           pf[n][m][1] = transpose8x8(FP8 ? pack_f16(w2, w3) : pack_bf16(w2, w3));
         }

@@ -17,8 +17,8 @@
 // 88: 256 * 192 + 128 * 40 + 128 * 88 = 65536.
 //
 // 8 bits: as in paged_attention.cu, codes enter the products as f16, a query row scaled by a power of two to at most 2^15, the key
-// scale of each 16 keys in the factor of the scores, the value scale 2^e in the weight 2^(s + e - M) and out of it in the sum
-// l = sum w 2^-e. With bf16 pages the factor is the softmax scale and e is 0. Keys that a sequence has no page for have e = -infinity.
+// scale of each 16 keys in the factor of the scores, the value scale 2^e in the weight w = 2^(s + e - M), beside the sum of 2^(s - M),
+// which is that of w 2^-e. With bf16 pages the factor is the softmax scale and e is 0. Keys that a sequence has no page for have e = -infinity.
 //
 // With few tiles the keys are split too: each of `splits` CTAs takes a part of the tile's blocks and leaves O (unnormalised, 32
 // bits), M and l; a second kernel adds them up in order.
@@ -448,8 +448,11 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
         if (grow) { l *= alpha; m_ref = m_new; }
       }
       const float nm = C::HEAD - (m_ref == -INFINITY ? 0.f : m_ref);
-      // (the FMA form of the exponential makes 2^-126 of -infinity: where there are masked keys, which have to weigh nothing even beside
-      // a sum of next to nothing, it is left out)
+      // Two forms. The FMA form of the exponential makes 2^-126 of -infinity, so it is left out where there are masked keys, which have to
+      // weigh nothing even beside a sum of next to nothing. And of pages far apart in scale the one's w is nothing beside the other's,
+      // its share of l is not: where a page is 2^80 below, l comes from the scores.
+#pragma unroll
+      for (int gp = 0; gp < 8; ++gp) masked |= FP8 && sc[gp].y + nm < -80.f;
       auto weights = [&](auto poly) {
         constexpr bool POLY = decltype(poly)::value;
 #pragma unroll
@@ -479,7 +482,14 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
             }
             float s0, s1;
             f2_unpack(sum2, s0, s1);
-            l = FP8 ? fmaf(s0 + s1, f.z, l) : l + (s0 + s1);
+if (FP8 && !POLY) {
+              if (f.z != 0.f) {
+#pragma unroll
+                for (int k = cc * 32 + hh * 16; k < cc * 32 + hh * 16 + 16; ++k) l += fast_exp2(fmaf(__uint_as_float(v[k]), fs, nm));
+              }
+            } else {
+              l = FP8 ? fmaf(s0 + s1, f.z, l) : l + (s0 + s1);
+            }
           }
           tmem_st_32x32b_x16(t_p + cc * 16, pk);
         }
