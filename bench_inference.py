@@ -30,6 +30,7 @@ def main() -> None:
     ap.add_argument("--preset", default="dense_7b_gqa")
     ap.add_argument("--layers", type=int, default=0, help="override the layer count (0 = preset); reported in config")
     ap.add_argument("--no-quant", action="store_true")
+    ap.add_argument("--kv-cache", choices=("paged", "paged_e4m3"), help="keys and values in pages, bf16 or 8 bits (one GPU; default: contiguous bf16)")
     a = ap.parse_args()
 
     import torch
@@ -59,7 +60,7 @@ def main() -> None:
 
     ttft, dec = [], []
     for rep in range(a.reps + 1):                       # first repetition is the warm-up
-        eng.reset(a.batch, a.prompt + a.decode + 8)
+        eng.reset(a.batch, a.prompt + a.decode + 8, a.kv_cache)
         if world > 1:
             dist.barrier()
         torch.cuda.synchronize()
@@ -86,7 +87,7 @@ def main() -> None:
             "data": "synthetic uniform tokens, random-init N(0,0.02) weights",
             "config": {"model": a.preset, "layers": cfg.num_layers, "weights": "bf16" if a.no_quant else "int4 g128 bf16 scales",
                        "batch": a.batch, "prompt": a.prompt, "decode": a.decode, "parallelism": f"tp{world}",
-                       "kv_cache": "bf16"},
+                       "kv_cache": {None: "bf16", "paged": "bf16 pages", "paged_e4m3": "e4m3 pages"}[a.kv_cache]},
             "sample_tokens": out[0, :8].tolist(), "device_error_word": native.read_error_flag()}))
     if world > 1:
         dist.barrier()

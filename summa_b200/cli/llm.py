@@ -53,6 +53,9 @@ def main(argv=None) -> int:
             p.add_argument("--top-k", type=int, default=0)
             p.add_argument("--repetition-penalty", type=float, default=1.0)
             p.add_argument("--seed", type=int, default=0)
+            if name == "generate":
+                p.add_argument("--kv-cache", choices=("paged", "paged_e4m3"),
+                               help="keys and values in pages, in the model's type or in 8 bits (default: one contiguous cache)")
         if name == "trace":
             p.add_argument("--output", "-o", required=True)
             p.add_argument("--metrics")
@@ -86,7 +89,7 @@ def main(argv=None) -> int:
     model, tok, cfg = _load(args)
     if args.cmd == "generate":
         from ..models.generate import SamplingConfig, TextGenerator
-        gen = TextGenerator(model, tok)
+        gen = TextGenerator(model, tok, kv_cache=args.kv_cache)
         text = gen.generate(args.prompt, SamplingConfig(max_new_tokens=args.max_new_tokens, temperature=args.temperature, top_k=args.top_k,
                                                         repetition_penalty=args.repetition_penalty, seed=args.seed,
                                                         stop_at_eos=not args.no_eos))

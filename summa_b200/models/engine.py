@@ -32,6 +32,7 @@ class InferenceEngine:
         self.device = model.embedding.weight.device
         self.use_graph = True
         self._graph = None
+        self._kv_cache = None
 
     @classmethod
     def build(cls, cfg, device: torch.device, tp_group=None, quantize: Optional[str] = "int4",
@@ -63,11 +64,31 @@ class InferenceEngine:
             raise ValueError(f"unknown quantisation `{quantize}`")
         return cls(model, tp)
 
-    def reset(self, batch: int, capacity: int):
-        """Start a new set of sequences. A state of the same shape is recycled (the KV caches are
+    def reset(self, batch: int, capacity: int, kv_cache: Optional[str] = None, num_pages: Optional[int] = None):
+        """Start a new set of sequences. `kv_cache`: None for one contiguous cache of one length, "paged" or "paged_e4m3" for pages in
+        the model's type or in 8 bits (`Transformer.make_paged_state`, with `num_pages` of it), which `prefill_ragged`, `release` and `decode`
+        then serve at the sequences' own lengths. A state of the same shape is recycled (the KV caches are
         overwritten as the new sequences grow, recurrent states start anew), which also keeps the captured decode graph."""
         st = self.state
-        if st is not None and st.capacity == capacity and st.layers \
+        if kv_cache is not None:
+            if self.tp is not None:
+                raise ValueError("the paged cache is not sharded: build the engine without a tensor-parallel group")
+            old = st.paged if st is not None else None
+            if old is not None and (old.batch, old.capacity, self._kv_cache) == (batch, capacity, kv_cache) \
+                    and old.num_pages == (batch * old.per_slot if num_pages is None else num_pages):
+                old.reset()
+                for i, l in enumerate(st.layers):
+                    if hasattr(l, "conv"):
+                        st.layers[i] = self.model.layers[i].ssm.make_state(batch, l.h.device, l.conv.dtype)
+                st.pos = 0
+                return
+            self.state = self.model.make_paged_state(batch, capacity, kv_cache, num_pages=num_pages)
+            self._kv_cache = kv_cache
+            self._graph = None
+            return
+        if num_pages is not None:
+            raise ValueError("num_pages belongs to a paged cache")
+        if st is not None and st.paged is None and st.capacity == capacity and st.layers \
                 and all((l.k if hasattr(l, "length") else l.conv).shape[0] == batch for l in st.layers):
             for i, l in enumerate(st.layers):
                 if hasattr(l, "length"):
@@ -92,11 +113,30 @@ class InferenceEngine:
         return ops.argmax(logits).view(-1, 1)
 
     @torch.no_grad()
+    def prefill_ragged(self, prompts) -> torch.Tensor:
+        """Brings a prompt of its own length to each slot of a paged state (None: nothing, the slot goes on as it is), so sequences
+        may join while others are being decoded. Returns the greedy next tokens `[B, 1]`; those of slots without a prompt are 0."""
+        if self.state is None or self.state.paged is None:
+            raise RuntimeError('call reset(batch, capacity, kv_cache="paged" or "paged_e4m3") first')
+        logits = self.model.forward_ragged_with_state(prompts, self.state)
+        brought = torch.tensor([p is not None and len(p) > 0 for p in prompts], device=logits.device)
+        return torch.where(brought, ops.argmax(logits), 0).view(-1, 1)
+
+    def release(self, slot: int) -> None:
+        """Ends the sequence of a slot of a paged state: its pages go back to the pool, and steps pass over the slot until it gets a prompt."""
+        if self.state is None or self.state.paged is None:
+            raise RuntimeError('call reset(batch, capacity, kv_cache="paged" or "paged_e4m3") first')
+        self.state.paged.release(slot)
+
+    @torch.no_grad()
     def decode(self, first: torch.Tensor, steps: int) -> torch.Tensor:
         """Greedy-decodes `steps` tokens after `first` `[B, 1]`; returns `[B, steps]` (the
-        tokens produced, not including `first`). No steps: an empty tensor, and the state stays as it is."""
+        tokens produced, not including `first`). No steps: an empty tensor, and the state stays as it is. Over a paged state every slot
+        in use goes on from its own length; what comes back for the others means nothing."""
         if steps < 0:
             raise ValueError(f"cannot decode {steps} tokens")
+        if self.state is not None and self.state.paged is not None and not any(self.state.paged.active()):
+            raise RuntimeError("no slot is in use: bring a prompt first")
         if steps == 0:
             return torch.empty(first.shape[0], 0, dtype=torch.long, device=first.device)
         if self.use_graph and self.device.type == "cuda" and not _has_hooks(self.model):
@@ -138,6 +178,9 @@ class _GraphDecoder:
             if blk.ssm is not None:
                 if not cuda_ops.mamba_decode_usable(blk.ssm):
                     return None
+            elif state.paged is not None:
+                if type(a) is not MultiHeadAttention or a.head_dim not in (64, 128):
+                    return None
             elif (not isinstance(a, MultiHeadAttention) or a.head_dim != 128 or a.window is not None or a.q_norm is not None
                     or not a.use_rope or not a.causal or a.num_heads // a.num_kv_heads > 8):
                 return None
@@ -154,8 +197,13 @@ class _GraphDecoder:
         self.ssm = [i for i, blk in enumerate(model.layers) if blk.ssm is not None]
         dev = model.embedding.weight.device
         st0 = state.layers[0]
-        self.B = (st0.conv if self.ssm and self.ssm[0] == 0 else st0.k).shape[0]
-        self.cap = state.layers[self.attn[0]].k.shape[1] if self.attn else state.capacity
+        self.paged = state.paged
+        if self.paged is not None:
+            self.B, self.cap = self.paged.batch, state.capacity
+            self.live = torch.zeros(self.B, dtype=torch.int32, device=dev)      # 1 for a slot in use: what a step adds to its length
+        else:
+            self.B = (st0.conv if self.ssm and self.ssm[0] == 0 else st0.k).shape[0]
+            self.cap = state.layers[self.attn[0]].k.shape[1] if self.attn else state.capacity
         # The captured step updates recurrent states of its own: a prefill leaves its results in fresh tensors, which `run`
         # copies in, and callers get copies back.
         self.rec = {i: (torch.empty_like(state.layers[i].conv, dtype=torch.bfloat16), torch.empty_like(state.layers[i].h))
@@ -164,7 +212,7 @@ class _GraphDecoder:
         self.pos = torch.zeros(1, dtype=torch.int32, device=dev)
         self.col = torch.zeros(1, 1, dtype=torch.long, device=dev)
         self.out = torch.zeros(self.B, max_steps, dtype=torch.long, device=dev)
-        if self.attn:                            # (the largest of the blocks: their head counts may differ)
+        if self.attn and self.paged is None:     # (the largest of the blocks: their head counts may differ)
             heads = {model.layers[i].attention.num_kv_heads for i in self.attn}
             self.splits = {k: native.call_value("sb_attention_decode_splits", self.B, k, self.cap) for k in heads}
             need = max(native.call_value("sb_attention_decode_workspace", self.B, k, n) for k, n in self.splits.items())
@@ -190,6 +238,8 @@ class _GraphDecoder:
                 from ..ops import cuda_ops
                 xz = self._norm_proj(blk.attn_norm, blk.ssm.in_proj, h)
                 h = self._proj_add(blk.ssm.out_proj, cuda_ops.mamba_decode_step(blk.ssm, xz, *self.rec[i]), h)
+            elif self.paged is not None:
+                h = self._attend_paged(blk, st, h, cos, sin)
             else:
                 h = self._attend(blk, st, h, cos, sin)
             ff = blk.feed_forward
@@ -205,6 +255,19 @@ class _GraphDecoder:
         native.call("sb_decode_pick", logits.data_ptr(), self.out.data_ptr(), B, logits.shape[1], logits.stride(0),
                     1 if logits.dtype == torch.bfloat16 else 0, self.tok.data_ptr(), self.col.data_ptr(), self.out.stride(0),
                     native.stream())
+        if self.paged is not None:
+            self.paged.lengths.add_(self.live)
+
+    def _attend_paged(self, blk, st, h, cos, sin):
+        """The attention branch of a block over its pages: every slot's position and length are read on the device."""
+        a = blk.attention
+        qkv = self._norm_proj(blk.attn_norm, a.qkv_proj, h)
+        rows = ops.PagedRows(self.paged.table, self.paged.lengths)
+        qg, kg = (a.q_norm.gamma, a.k_norm.gamma) if a.q_norm is not None else (None, None)
+        rope = (cos, sin) if a.use_rope else (None, None)
+        q = ops.paged_append(qkv, qg, kg, a.eps, *rope, a.num_heads, a.num_kv_heads, a.head_dim, st.kv, rows)
+        o = ops.paged_attention(q, st.kv, rows, a.causal, a.window)
+        return self._proj_add(a.o_proj, o.view(self.B, a.q_dim), h)
 
     def _attend(self, blk, st, h, cos, sin):
         """The attention branch of a block with its residual: qkv projection, RoPE, cache append, split-KV attention, o_proj."""
@@ -286,8 +349,14 @@ class _GraphDecoder:
         self.graph = g
 
     def run(self, first: torch.Tensor, steps: int) -> torch.Tensor:
-        start = self.state.layers[self.attn[0]].length if self.attn else self.state.pos
-        if self.attn and start + steps > self.cap:
+        if self.paged is not None:
+            live = [int(on) for on in self.paged.active()]
+            self.paged.reserve([steps * on for on in live])
+            self.live.copy_(torch.tensor(live, dtype=torch.int32))
+            start = self.state.pos
+        else:
+            start = self.state.layers[self.attn[0]].length if self.attn else self.state.pos
+        if self.paged is None and self.attn and start + steps > self.cap:
             raise RuntimeError(f"KV cache overflow: {start + steps} > capacity {self.cap}")
         for i, (conv, hid) in self.rec.items():
             conv.copy_(self.state.layers[i].conv)
@@ -305,8 +374,11 @@ class _GraphDecoder:
                 self._capture(torch.cuda.memory_stats().get(allocated, 0) - before)
         for _ in range(steps - done):
             self.graph.replay()
-        for i in self.attn:
-            self.state.layers[i].length = start + steps
+        if self.paged is not None:
+            self.paged.advance([steps * on for on in live], on_device=False)
+        else:
+            for i in self.attn:
+                self.state.layers[i].length = start + steps
         for i, (conv, hid) in self.rec.items():
             self.state.layers[i].conv = conv.to(self.state.layers[i].conv.dtype, copy=True)
             self.state.layers[i].h = hid.clone()

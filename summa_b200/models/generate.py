@@ -26,10 +26,15 @@ class SamplingConfig:
 
 
 class TextGenerator:
-    def __init__(self, model, tokenizer=None, eos_id: Optional[int] = None):
+    def __init__(self, model, tokenizer=None, eos_id: Optional[int] = None, kv_cache: Optional[str] = None):
+        """`kv_cache`: None for the contiguous cache, or "paged" / "paged_e4m3" (`Transformer.make_paged_state`)."""
         self.model = model
         self.tokenizer = tokenizer
         self.eos_id = eos_id if eos_id is not None else (tokenizer.eos_id() if tokenizer is not None else None)
+        self.kv_cache = kv_cache
+
+    def _state(self, capacity: int):
+        return self.model.make_state(1, capacity) if self.kv_cache is None else self.model.make_paged_state(1, capacity, self.kv_cache)
 
     @torch.no_grad()
     def generate_ids(self, prompt: List[int], cfg: SamplingConfig) -> List[int]:
@@ -44,7 +49,7 @@ class TextGenerator:
         gen = torch.Generator(device="cpu").manual_seed(cfg.seed)
         tokens = list(prompt)
         out: List[int] = []
-        state = model.make_state(1, capacity)
+        state = self._state(capacity)
         logits = model.forward_next_logits_with_state(torch.tensor([tokens], device=dev), state)
         for _ in range(cfg.max_new_tokens):
             nxt = self._select(logits[0], tokens, cfg, gen)
@@ -57,7 +62,7 @@ class TextGenerator:
             if state.pos + 1 > capacity:
                 keep = tokens[-(max_len // 2):]
                 capacity = min(max_len, len(keep) + cfg.max_new_tokens - len(out))
-                state = model.make_state(1, capacity)
+                state = self._state(capacity)
                 logits = model.forward_next_logits_with_state(torch.tensor([keep], device=dev), state)
             else:
                 logits = model.forward_next_logits_with_state(torch.tensor([[nxt]], device=dev), state)

@@ -22,6 +22,7 @@ from ..mal import BlockDef, ModelDef
 from .layers import (AttentionState, FeedForward, Linear, MambaMixer, MambaState,
                      MultiHeadAttention, Norm, SparseMoe, build_ffn)
 from .memory import MemoryChain
+from .paged import PAGE, PagedCache
 
 EMBEDDING_INIT_STD = 0.02
 LOSS_CHUNKS = 4
@@ -184,6 +185,7 @@ class InferenceState:
     layers: list
     pos: int = 0
     capacity: int = 0
+    paged: Optional[PagedCache] = None       # the slots' lengths and pages, where the attention layers' cache is paged
 
 
 class _GradReady(torch.autograd.Function):
@@ -387,13 +389,79 @@ class Transformer(nn.Module):
                 layers.append(blk.attention.make_state(batch, capacity, p.device, dtype))
         return InferenceState(layers, 0, capacity)
 
+    def make_paged_state(self, batch: int, capacity: Optional[int] = None, kv_cache: str = "paged", page: int = PAGE,
+                         num_pages: Optional[int] = None, dtype=None) -> InferenceState:
+        """State whose attention layers keep keys and values in pages (`models.paged`), so that sequences differ in length: in the
+        model's type (`kv_cache="paged"`) or in 8 bits with a scale per page and head (`"paged_e4m3"`). The batch's slots are out of use until
+        a forward pass brings rows to them."""
+        capacity = capacity or self.cfg.max_seq_len
+        if capacity > self.cfg.max_seq_len and self.rope(self.embedding.weight.device) is not None:
+            raise ValueError(f"capacity {capacity} beyond max_seq_len {self.cfg.max_seq_len}")
+        p = self.embedding.weight
+        dtype = dtype or (self.stream_dtype or p.dtype)
+        cache = PagedCache(batch, capacity, page, num_pages, p.device)
+        layers = []
+        for blk in self.layers:
+            if blk.ssm is not None:
+                layers.append(blk.ssm.make_state(batch, p.device, dtype))
+            else:
+                layers.append(cache.layer(blk.attention.num_kv_heads, blk.attention.head_dim, dtype, kv_cache))
+        return InferenceState(layers, 0, capacity, cache)
+
     def forward_hidden_with_state(self, tokens: torch.Tensor, state: InferenceState) -> torch.Tensor:
+        """Over a paged state (no gradients) the rows go to the slots in use, or to all where none is yet."""
+        grow = None
+        if state.paged is not None:
+            live = state.paged.active()
+            if not any(live):
+                live = [True] * len(live)
+            elif not all(live) and tokens.shape[1] != 1:
+                raise ValueError("some slots are not in use: bring their prompts with forward_ragged_with_state")
+            if len(live) != tokens.shape[0]:
+                raise ValueError(f"{tokens.shape[0]} rows for a state of {len(live)} slots")
+            grow = [tokens.shape[1] if on else 0 for on in live]
+            state.paged.begin(grow) if all(live) else state.paged.begin_step(grow)
         x = self.embed(tokens)
         rope = self.rope(tokens.device)
         for blk, st in zip(self.layers, state.layers):
             x, _ = blk(x, rope, st, None)
+        if grow is not None:
+            state.paged.advance(grow)
         state.pos += tokens.shape[1]
         return self.final_norm(x)
+
+    @torch.no_grad()
+    def forward_ragged_with_state(self, prompts: Sequence[Optional[Sequence[int]]], state: InferenceState) -> torch.Tensor:
+        """Brings `prompts[b]` to slot b of a paged state, each of its own length and behind whatever the slot holds (None or empty: nothing).
+        Logits `[B, vocab_size]` at each prompt's last token; rows of slots without a prompt are zeros."""
+        if state.paged is None:
+            raise ValueError("prompts of different lengths need a paged state (make_paged_state)")
+        if any(blk.ssm is not None for blk in self.layers):
+            raise ValueError("recurrent layers take prompts of one length")
+        prompts = [p if p is not None else () for p in prompts]
+        grow = [len(p) for p in prompts]
+        if len(grow) != state.paged.batch:
+            raise ValueError(f"{len(grow)} prompts for {state.paged.batch} slots")
+        dev = self.embedding.weight.device
+        logits = torch.zeros(len(grow), self.cfg.vocab_size, dtype=self.stream_dtype or self.embedding.weight.dtype, device=dev)
+        if not any(grow):
+            return logits
+        flat = torch.cat([torch.as_tensor(p, dtype=torch.long, device=dev).reshape(-1) for p in prompts])[None]
+        state.paged.begin(grow)
+        x = self.embed(flat)
+        rope = self.rope(dev)
+        for blk, st in zip(self.layers, state.layers):
+            x, _ = blk(x, rope, st, None)
+        state.paged.advance(grow)
+        at, last, slots = 0, [], []
+        for b, n in enumerate(grow):
+            at += n
+            if n:
+                last.append(at - 1)
+                slots.append(b)
+        rows = self.project_logits(self.final_norm(x[0, torch.tensor(last, device=dev)]))
+        logits[torch.tensor(slots, device=dev)] = rows.to(logits.dtype)
+        return logits
 
     def forward_with_state(self, tokens: torch.Tensor, state: InferenceState) -> torch.Tensor:
         x = self.forward_hidden_with_state(tokens, state)
