@@ -5,16 +5,18 @@
 // in tensor memory. A tile is 256 (row, head) pairs of one sequence and one kv head, rows first: pair x is row x / G, query head x % G.
 // All heads that share the kv head ride in one tile, so the keys and values that it takes from the cache, and expands, serve G times
 // the rows, and a short chunk fills the tile. Two groups of 128 pairs take turns on the tensor core:
-//   warps 0-3 / 4-7   a thread per pair: its query row to shared memory, then per block of 128 keys its scores from tensor memory,
+//   warps 0-3 / 4-7   a thread per pair: its query row to shared memory, then per block of 64 keys its scores from tensor memory,
 //                     masks, running maximum, weights back into tensor memory as operand A of the next product; at the end its output row
 //   warp 8            issues S = Q K^T
 //   warp 9            issues O += P V
 //   warps 12-15       bring keys and values from their pages into the swizzled tiles that the products read: bf16 as 16-byte
 //                     asynchronous copies, e4m3 through registers, where it becomes f16
+// A group has two score buffers of 64 columns, each with its weights in place, so the scores of the next block are computed while the
+// threads are at this one, and they wait for a product only where their maximum makes them rescale O. (With one buffer of 128 columns a
+// block took 6500 cycles, 2300 of them each group's wait for its two products.) Products of 64 columns cost 45 cycles where 128 cost 64:
+// 2464 cycles of the tensor core for 128 keys and 256 pairs instead of 2048, but it was busy a third of the time.
 // (A bulk tensor copy could fetch bf16 pages, but not expand codes, nor leave out single rows of a page that hold nothing yet: what
-// lies behind a sequence's last row may be NaN, and 0 * NaN would reach its sums.) The register file is split by setmaxnreg: 512
-// threads start with 128 registers each, 65536 in all; 256 softmax threads take 192, the issuing warpgroup keeps 40 and the copying one
-// 88: 256 * 192 + 128 * 40 + 128 * 88 = 65536.
+// lies behind a sequence's last row may be NaN, and 0 * NaN would reach its sums.)
 //
 // 8 bits: as in paged_attention.cu, codes enter the products as f16, a query row scaled by a power of two to at most 2^15, the key
 // scale of each 16 keys in the factor of the scores, the value scale 2^e in the weight w = 2^(s + e - M), beside the sum of 2^(s - M),
@@ -46,25 +48,32 @@ struct PagedPrefillParams {
   unsigned int* err;
 };
 
-constexpr int PP_THREADS = 512;
+#ifndef PP_POLY
+#define PP_POLY 8
+#endif
+constexpr int PP_THREADS = 512, PP_KEYS = 64;
 template <int D, bool FP8>
 struct PagedPrefill {
-  static constexpr bool SEP = D == 64;                           // weights in tensor memory columns of their own
-  static constexpr int TILE = 128 * D * 2;
-  static constexpr int NSK = D == 64 ? 3 : 2, NSV = NSK;
-  static constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + NSK * TILE, OFF_SCALE = OFF_V + NSV * TILE;
+  static constexpr int TILE = 128 * D * 2, KTILE = PP_KEYS * D * 2;
+  static constexpr int NS = 4;                                   // stages of keys and of values
+  static constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + NS * KTILE, OFF_SCALE = OFF_V + NS * KTILE;
   static constexpr int RING = 8;                                 // blocks whose scales are kept: more than can be under way
-  static constexpr int OFF_BAR = OFF_SCALE + RING * 8 * 16;
+  static constexpr int OFF_BAR = OFF_SCALE + RING * 4 * 16;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
-  static constexpr int COL_S = 0, COL_O = 256, COL_P = SEP ? 384 : 0, P_STRIDE = SEP ? 64 : 128;
+  static constexpr int COL_O = 256;                              // S (and P in place) of group a, buffer b at a * 128 + b * 64
   static constexpr int CPR = (FP8 ? D : 2 * D) / 16;             // 16-byte chunks of a key
-  static constexpr int LOADS = 128 * CPR / 128;                  // of a copying thread, per tile of 128 keys
+  static constexpr int LOADS = PP_KEYS * CPR / 128;              // of a copying thread, per tile of 64 keys
   static constexpr float HEAD = FP8 ? 9.f : 0.f, SLACK = FP8 ? 6.f : 8.f;
 };
 
 // f16 operands: as make_idesc_bf16, formats 0
 __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, int a_mn_major, int b_mn_major) {
   return make_idesc_bf16(M, N, a_mn_major, b_mn_major) & ~((1u << 7) | (1u << 10));
+}
+
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 struct PrefillTile {
@@ -110,23 +119,23 @@ __device__ __forceinline__ PrefillTile prefill_tile(const PagedBatch& p, int G, 
 template <int D, bool FP8>
 __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const PagedPrefillParams p) {
   using C = PagedPrefill<D, FP8>;
-  constexpr int NSK = C::NSK, NSV = C::NSV;
+  constexpr int NS = C::NS;
   extern __shared__ uint8_t smem_raw[];
   asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  uint64_t* q_full = bars + 0;    // 256 arrivals
-  uint64_t* s_full = bars + 1;    // [2]
-  uint64_t* s_free = bars + 3;    // [2], 128 arrivals: the group has read S (SEP only)
-  uint64_t* p_full = bars + 5;    // [2], 128 arrivals
-  uint64_t* o_full = bars + 7;    // [2] the product of a block is complete
-  uint64_t* k_full = bars + 9;    // [NSK], 128 arrivals
-  uint64_t* k_empty = bars + 12;
-  uint64_t* v_full = bars + 15;   // [NSV], 128 arrivals
-  uint64_t* v_empty = bars + 18;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  // (where threads arrive, a warp's have fenced what they did, and one of them does)
+  uint64_t* q_full = bars + 0;    // 8 arrivals
+  uint64_t* s_full = bars + 1;    // [2 groups][2 buffers]
+  uint64_t* p_full = bars + 5;    // [2][2], 4 arrivals
+  uint64_t* o_full = bars + 9;    // [2][2] the product with a buffer's weights is complete (one for each buffer: who waits is a phase behind at most)
+  uint64_t* k_full = bars + 13;   // [NS], 4 arrivals
+  uint64_t* k_empty = bars + 17;
+  uint64_t* v_full = bars + 21;   // [NS], 4 arrivals
+  uint64_t* v_empty = bars + 25;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float4* scales = reinterpret_cast<float4*>(smem + C::OFF_SCALE);       // [RING][8]: key factor, e, 2^-e
+  float4* scales = reinterpret_cast<float4*>(smem + C::OFF_SCALE);       // [RING][4]: key factor, e, 2^-e
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kh = blockIdx.x;
@@ -154,7 +163,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     else if (p.window >= 0) hi = static_cast<int>(min(static_cast<long>(hi), static_cast<long>(tl.len) + last_row + p.window + 1));
     if (p.window >= 0) lo = static_cast<int>(max(static_cast<long>(tl.len) + first_row - p.window, 0L));
   }
-  int j0 = lo / 128, j1 = (hi + 127) / 128;
+  int j0 = lo / PP_KEYS, j1 = (hi + PP_KEYS - 1) / PP_KEYS;       // blocks of keys
   if (hi <= lo) j1 = j0;
   if (p.splits > 1) {
     const int per = (j1 - j0 + p.splits - 1) / p.splits, end = j1;
@@ -164,12 +173,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
   const int nblk = j1 - j0;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 256);
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(&s_full[a], 1); mbar_init(&s_free[a], 128); mbar_init(&p_full[a], 128); mbar_init(&o_full[a], 1);
-    }
-    for (int s = 0; s < 3; ++s) {
-      mbar_init(&k_full[s], 128); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 128); mbar_init(&v_empty[s], 1);
+    mbar_init(q_full, 8);
+    for (int s = 0; s < 4; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&k_full[s], 4); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 4); mbar_init(&v_empty[s], 1);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -182,133 +189,148 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
 
   if (warp >= 12) {
     // ---------------------------------------------------------------- copies
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     const int tid = threadIdx.x - 384, shift = p.batch.page_shift, mask = (1 << shift) - 1;
     const int* table = p.batch.table + tl.b * p.batch.table_ld;
-    const uint8_t *kb = p.k + kh * p.k_head, *vb = p.v + kh * p.v_head;
-    // chunk i of a thread: row r(i), chunk c of the row; 16 keys of one page share a look-up
-    constexpr int RPI = 128 / C::CPR, IDS = RPI >= 16 ? C::LOADS : 8;     // rows of a step, pages that a thread meets in a tile
+    // chunk i of a thread: row i * RPI + r0 of the tile, chunk c of the row
+    constexpr int RPI = 128 / C::CPR, LOADS = C::LOADS, IDS = RPI >= 16 ? LOADS : 4;   // IDS: pages that a thread meets in a tile
     const int r0 = tid / C::CPR, c = tid % C::CPR;
-    auto row_of = [&](int i) { return i * RPI + r0; };
-    int id[IDS] = {}, next[IDS];
-    auto look_up = [&](int j, int* to) {
+    const uint8_t *kb = p.k + kh * p.k_head + c * 16, *vb = p.v + kh * p.v_head + c * 16;
+    int id[IDS], next[IDS];
+    auto look_up = [&](int j) {
 #pragma unroll
       for (int i = 0; i < IDS; ++i) {
-        const int key = j * 128 + (RPI >= 16 ? row_of(i) : i * 16);
-        to[i] = -2;
-        if (j < j1 && (key | 15) >= lo && (key & ~15) < hi) to[i] = table[key >> shift];
+        const int key = j * PP_KEYS + (RPI >= 16 ? i * RPI + r0 : i * 16);
+        next[i] = -2;
+        if (j < j1 && (key | 15) >= lo && (key & ~15) < hi) next[i] = table[key >> shift];
       }
     };
     auto source = [&](const uint8_t* base, long stride, int i, int j, bool* in) -> const uint8_t* {
-      const int page = id[RPI >= 16 ? i : i * RPI / 16], key = j * 128 + row_of(i);
+      const int page = id[RPI >= 16 ? i : i * RPI / 16], key = j * PP_KEYS + i * RPI + r0;
       *in = static_cast<unsigned>(page) < static_cast<unsigned>(p.batch.num_pages) && key >= lo && key < hi;
-      return base + (*in ? static_cast<uint64_t>(page) * static_cast<uint32_t>(stride) + static_cast<uint32_t>((key & mask) * (C::CPR * 16) + c * 16) : 0);
+      return base + (*in ? static_cast<uint64_t>(page) * static_cast<uint32_t>(stride) + static_cast<uint32_t>((key & mask) * (C::CPR * 16)) : 0);
     };
-    // where 8 elements (16 bytes) of row r, elements 8 e .. lie in a tile: 64 elements a row of a swizzled half
-    auto place = [&](int r, int e) -> uint32_t { return (e >> 3) * 16384 + r * 128 + (((e & 7) ^ (r & 7)) << 4); };
-    bool ok = true;
-    uint4 raw[FP8 ? C::LOADS : 1];
-    look_up(j0, next);
-    for (int n = 0; n < 2 * nblk && ok; ++n) {                   // K and V of block 0, of block 1, ...
-      const int i = n >> 1, j = j0 + i;
-      const bool is_v = n & 1;
-      if (!is_v) {
-#pragma unroll
-        for (int x = 0; x < IDS; ++x) id[x] = next[x];
-        look_up(j + 1, next);
-        // the scales of its groups of 16 keys, read by the softmax threads behind S
-        if (tid < 8) {
-          const int key = j * 128 + tid * 16;
-          int page = -1;
-          if (key + 16 > lo && key < hi) {
-            page = table[key >> shift];
-            if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.batch.num_pages)) { page = -1; atomicOr(p.err, 4u); }
-          }
-          float4 f = make_float4(1.f, page >= 0 ? 0.f : -INFINITY, page >= 0 ? 1.f : 0.f, 0.f);
-          if (FP8 && page >= 0) {
-            const int e = min(max(scale_exp(p.vs[page * p.vs_ld + kh]), PAGED_LEAST_EXP), PAGED_MOST_EXP);
-            f = make_float4(p.ks[page * p.ks_ld + kh], static_cast<float>(e), exp_scale(-e), 0.f);
-          }
-          scales[(i % C::RING) * 8 + tid] = f;
+    // where elements 8 e .. 8 e + 7 of row r lie in a tile: 64 elements a row of a swizzled half
+    auto place = [&](int r, int e) -> uint32_t { return (e >> 3) * (PP_KEYS * 128) + r * 128 + (((e & 7) ^ (r & 7)) << 4); };
+    // the scales of block j's groups of 16 keys, read by the softmax threads behind S
+    auto put_scales = [&](int i, int j) {
+      if (tid < 4) {
+        const int key = j * PP_KEYS + tid * 16;
+        int page = -1;
+        if (key + 16 > lo && key < hi) {
+          page = table[key >> shift];
+          if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.batch.num_pages)) { page = -1; atomicOr(p.err, 4u); }
         }
+        float4 f = make_float4(1.f, 0.f, page >= 0 ? 1.f : 0.f, 0.f);
+        if (FP8 && page >= 0) {
+          const int e = min(max(scale_exp(p.vs[page * p.vs_ld + kh]), PAGED_LEAST_EXP), PAGED_MOST_EXP);
+          f = make_float4(p.ks[page * p.ks_ld + kh], static_cast<float>(e), exp_scale(-e), 0.f);
+        }
+        scales[(i % C::RING) * 4 + tid] = f;
       }
-      const int s = i % (is_v ? NSV : NSK);
-      uint8_t* dst = smem + (is_v ? C::OFF_V : C::OFF_K) + s * C::TILE;
-      const uint8_t* base = is_v ? vb : kb;
-      const long stride = is_v ? p.v_page : p.k_page;
-      if (FP8) {
+    };
+    bool ok = true;
+    look_up(j0);
+    if (FP8) {
+      uint4 rk[LOADS], rv[LOADS];
+      auto load = [&](uint4* r, const uint8_t* base, long stride, int j) {
 #pragma unroll
-        for (int x = 0; x < C::LOADS; ++x) {
+        for (int x = 0; x < LOADS; ++x) {
           bool in;
           const uint8_t* src = source(base, stride, x, j, &in);
-          raw[x] = make_uint4(0, 0, 0, 0);
-          if (in) raw[x] = *reinterpret_cast<const uint4*>(src);
+          r[x] = make_uint4(0, 0, 0, 0);
+          if (in) r[x] = *reinterpret_cast<const uint4*>(src);
         }
-      }
-      ok = mbar_wait(is_v ? &v_empty[s] : &k_empty[s], ((i / (is_v ? NSV : NSK)) & 1) ^ 1, abort_flag, p.err);
-      if (!ok) break;
-      if (FP8) {
+      };
+      auto store = [&](const uint4* r, uint8_t* dst) {
 #pragma unroll
-        for (int x = 0; x < C::LOADS; ++x) {
-          const uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+        for (int x = 0; x < LOADS; ++x) {
+          const uint32_t w[4] = {r[x].x, r[x].y, r[x].z, r[x].w};
           uint32_t h[8];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
                 : "=r"(h[2 * k]), "=r"(h[2 * k + 1]) : "r"(w[k]));
-          const int r = row_of(x);
-          *reinterpret_cast<uint4*>(dst + place(r, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4*>(dst + place(r, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+          *reinterpret_cast<uint4*>(dst + place(x * RPI + r0, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(dst + place(x * RPI + r0, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
         }
         fence_proxy_async_smem();
-        mbar_arrive(is_v ? &v_full[s] : &k_full[s]);
-      } else {
+      };
+      auto turn = [&](int j) {
 #pragma unroll
-        for (int x = 0; x < C::LOADS; ++x) {
+        for (int x = 0; x < IDS; ++x) id[x] = next[x];
+        look_up(j + 1);
+      };
+      turn(j0);
+      if (nblk > 0) load(rk, kb, p.k_page, j0);
+      for (int i = 0; i < nblk && ok; ++i) {
+        const int s = i % NS;
+        load(rv, vb, p.v_page, j0 + i);
+        put_scales(i, j0 + i);
+        ok = mbar_wait(&k_empty[s], ((i / NS) & 1) ^ 1, abort_flag, p.err);
+        if (!ok) break;
+        store(rk, smem + C::OFF_K + s * C::KTILE);
+        warp_arrive(&k_full[s]);
+        turn(j0 + i + 1);
+        if (i + 1 < nblk) load(rk, kb, p.k_page, j0 + i + 1);
+        ok = mbar_wait(&v_empty[s], ((i / NS) & 1) ^ 1, abort_flag, p.err);
+        if (!ok) break;
+        store(rv, smem + C::OFF_V + s * C::KTILE);
+        warp_arrive(&v_full[s]);
+      }
+    } else {
+      // tiles in the order K of block 0, V of block 0, K of block 1, ...; one is handed over when the two behind it are under way
+      auto full = [&](int n) { return (n & 1) ? &v_full[(n >> 1) % NS] : &k_full[(n >> 1) % NS]; };
+      for (int n = 0; n < 2 * nblk && ok; ++n) {
+        const int i = n >> 1, j = j0 + i, s = i % NS;
+        const bool is_v = n & 1;
+        if (!is_v) {
+#pragma unroll
+          for (int x = 0; x < IDS; ++x) id[x] = next[x];
+          look_up(j + 1);
+          put_scales(i, j);
+        }
+        ok = mbar_wait(is_v ? &v_empty[s] : &k_empty[s], ((i / NS) & 1) ^ 1, abort_flag, p.err);
+        if (!ok) break;
+        uint8_t* dst = smem + (is_v ? C::OFF_V : C::OFF_K) + s * C::KTILE;
+#pragma unroll
+        for (int x = 0; x < LOADS; ++x) {
           bool in;
-          const uint8_t* src = source(base, stride, x, j, &in);
-          cp_async16_zfill(smem_u32(dst + place(row_of(x), c)), src, in ? 16 : 0);
+          const uint8_t* src = source(is_v ? vb : kb, is_v ? p.v_page : p.k_page, x, j, &in);
+          cp_async16_zfill(smem_u32(dst + place(x * RPI + r0, c)), src, in ? 16 : 0);
         }
         cp_async_commit();
-        // the tile before this one has landed: hand it over
-        if (n > 0) {
-          cp_async_wait_group<1>();
+        if (n >= 2) {
+          cp_async_wait_group<2>();
           fence_proxy_async_smem();
-          const int i1 = (n - 1) >> 1;
-          mbar_arrive(is_v ? &k_full[i1 % NSK] : &v_full[i1 % NSV]);
+          warp_arrive(full(n - 2));
         }
       }
-    }
-    if (!FP8) {
       cp_async_wait_group<0>();
       if (ok && nblk > 0) {
         fence_proxy_async_smem();
-        mbar_arrive(&v_full[(nblk - 1) % NSV]);
+        warp_arrive(full(2 * nblk - 2));
+        warp_arrive(full(2 * nblk - 1));
       }
     }
   } else if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 8 && lane == 0 && nblk > 0) {
       // -------------------------------------------------------------- S = Q K^T
-      constexpr uint32_t idesc = FP8 ? make_idesc_f16(128, 128, 0, 0) : make_idesc_bf16(128, 128, 0, 0);
+      constexpr uint32_t idesc = FP8 ? make_idesc_f16(128, PP_KEYS, 0, 0) : make_idesc_bf16(128, PP_KEYS, 0, 0);
       const uint32_t q_base = smem_u32(smem), k_base = smem_u32(smem + C::OFF_K);
       bool ok = mbar_wait(q_full, 0, abort_flag, p.err);
       for (int i = 0; i < nblk && ok; ++i) {
-        const int ks = i % NSK;
-        if (!mbar_wait(&k_full[ks], (i / NSK) & 1, abort_flag, p.err)) break;
+        const int ks = i % NS, b = i & 1;
+        if (!mbar_wait(&k_full[ks], (i / NS) & 1, abort_flag, p.err)) break;
         for (int a = 0; a < tiles_here && ok; ++a) {
-          if (i > 0) {
-            ok = C::SEP ? mbar_wait(&s_free[a], (i - 1) & 1, abort_flag, p.err) : mbar_wait(&o_full[a], (i - 1) & 1, abort_flag, p.err);
-            if (!ok) break;
-          }
+          // the buffer held the weights of block i - 2
+          if (i > 1) ok = mbar_wait(&o_full[a * 2 + b], ((i - 2) >> 1) & 1, abort_flag, p.err);
+          if (!ok) break;
           tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-            umma_bf16(tmem_base + C::COL_S + a * 128, make_smem_desc_sw128(q_base + a * C::TILE + off, 16, 1024),
-                      make_smem_desc_sw128(k_base + ks * C::TILE + off, 16, 1024), idesc, kk > 0 ? 1u : 0u);
-          }
-          umma_commit(&s_full[a]);
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_bf16(tmem_base + a * 128 + b * 64, make_smem_desc_sw128(q_base + a * C::TILE + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024),
+                      make_smem_desc_sw128(k_base + ks * C::KTILE + (kk >> 2) * (PP_KEYS * 128) + (kk & 3) * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+          umma_commit(&s_full[a * 2 + b]);
         }
         if (ok) umma_commit(&k_empty[ks]);
       }
@@ -318,16 +340,16 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       const uint32_t v_base = smem_u32(smem + C::OFF_V);
       bool ok = true;
       for (int i = 0; i < nblk && ok; ++i) {
-        const int vs = i % NSV;
-        if (!mbar_wait(&v_full[vs], (i / NSV) & 1, abort_flag, p.err)) break;
+        const int vs = i % NS, b = i & 1;
+        if (!mbar_wait(&v_full[vs], (i / NS) & 1, abort_flag, p.err)) break;
         for (int a = 0; a < tiles_here && ok; ++a) {
-          if (!mbar_wait(&p_full[a], i & 1, abort_flag, p.err)) { ok = false; break; }
+          if (!mbar_wait(&p_full[a * 2 + b], (i >> 1) & 1, abort_flag, p.err)) { ok = false; break; }
           tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_bf16_ta(tmem_base + C::COL_O + a * D, tmem_base + C::COL_P + a * C::P_STRIDE + 8 * kk,
-                         make_smem_desc_sw128(v_base + vs * C::TILE + kk * 2048, 16384, 1024), idesc, (i > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&o_full[a]);
+          for (int kk = 0; kk < PP_KEYS / 16; ++kk)
+            umma_bf16_ta(tmem_base + C::COL_O + a * D, tmem_base + a * 128 + b * 64 + 8 * kk,
+                         make_smem_desc_sw128(v_base + vs * C::KTILE + kk * 2048, PP_KEYS * 128, 1024), idesc, (i > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&o_full[a * 2 + b]);
         }
         if (ok) umma_commit(&v_empty[vs]);
       }
@@ -335,15 +357,12 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax, a thread per pair
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int a = warp >> 2, t = threadIdx.x & 127;
     const long x = x0 + a * 128 + t;
     const bool live = x < pairs;
     const int row = live ? static_cast<int>(x / p.G) : 0, head = kh * p.G + (live ? static_cast<int>(x % p.G) : 0);
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem_base + C::COL_S + a * 128 + lane_sel;
     const uint32_t t_o = tmem_base + C::COL_O + a * D + lane_sel;
-    const uint32_t t_p = tmem_base + C::COL_P + a * C::P_STRIDE + lane_sel;
 
     // the query row into its tile; in 8 bits as f16, scaled by a power of two
     float back = p.scale_log2;
@@ -382,7 +401,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(tile + (i >> 3) * 16384 + t * 128 + (((i & 7) ^ (t & 7)) << 4)) = w[i];
       fence_proxy_async_smem();
-      mbar_arrive(q_full);
+      warp_arrive(q_full);
     }
 
     // keys that this pair sees: [klo, khi)
@@ -396,81 +415,86 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     if (!live) khi = 0;
     float m_ref = -INFINITY, l = 0.f;
     bool ok = a < tiles_here;
-    const bool group = ok;
+#pragma unroll 1
     for (int i = 0; i < nblk && ok; ++i) {
-      const int kv0 = (j0 + i) * 128;
-      if (!mbar_wait(&s_full[a], i & 1, abort_flag, p.err)) { ok = false; break; }
+      const int kv0 = (j0 + i) * PP_KEYS, b = i & 1;
+      const uint32_t t_s = tmem_base + a * 128 + b * 64 + lane_sel;
+      if (!mbar_wait(&s_full[a * 2 + b], (i >> 1) & 1, abort_flag, p.err)) { ok = false; break; }
       tc_fence_after();
-      uint32_t v[128];
+      uint32_t v[64];
       tmem_ld_32x32b_x32(t_s, v);
       tmem_ld_32x32b_x32(t_s + 32, v + 32);
-      tmem_ld_32x32b_x32(t_s + 64, v + 64);
-      tmem_ld_32x32b_x32(t_s + 96, v + 96);
-      tmem_ld_wait();
-      if (C::SEP) {
-        tc_fence_before();
-        mbar_arrive(&s_free[a]);
+      // factor and exponent of the four groups of 16 keys (bf16 pages: the softmax scale and 0)
+      const uint32_t sc = smem_u32(scales) + (i % C::RING) * 64;
+      float fs[4], e[4], inv[4];
+      bool masked = kv0 < klo || kv0 + PP_KEYS > khi;
+#pragma unroll
+      for (int gp = 0; gp < 4; ++gp) {
+        float unused;
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(fs[gp]), "=f"(e[gp]), "=f"(inv[gp]), "=f"(unused) : "r"(sc + gp * 16) : "memory");
+        masked |= inv[gp] == 0.f;              // a page is missing
+        fs[gp] = FP8 ? fs[gp] * back : back;
       }
-      const float4* sc = scales + (i % C::RING) * 8;
-      bool masked = kv0 < klo || kv0 + 128 > khi;
+      tmem_ld_wait();
       if (masked) {
         const int from = klo - kv0, to = khi - kv0;
 #pragma unroll
-        for (int k = 0; k < 128; ++k) v[k] = (k >= from && k < to) ? v[k] : 0xff800000u;   // -inf
+        for (int k = 0; k < 64; ++k) v[k] = (k >= from && k < to && inv[k >> 4] != 0.f) ? v[k] : 0xff800000u;   // -inf
+#pragma unroll
+        for (int gp = 0; gp < 4; ++gp) fs[gp] = fmaxf(fs[gp], 1e-37f);     // (-inf times what has underflown to 0 would be NaN)
       }
       float m_blk = -INFINITY;
 #pragma unroll
-      for (int gp = 0; gp < 8; ++gp) {
+      for (int gp = 0; gp < 4; ++gp) {
         float mx = -INFINITY;
 #pragma unroll
         for (int k = 0; k < 16; k += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(v[gp * 16 + k]), __uint_as_float(v[gp * 16 + k + 1])));
-        const float4 f = sc[gp];
-        m_blk = fmaxf(m_blk, fmaf(mx, fmaxf(back * f.x, 1e-37f), f.y));
-        masked |= f.z == 0.f;
+        m_blk = fmaxf(m_blk, FP8 ? fmaf(mx, fs[gp], e[gp]) : mx * fs[gp]);
       }
       const bool grow = m_blk > m_ref + C::SLACK;
-      if (i > 0 && !mbar_wait(&o_full[a], (i - 1) & 1, abort_flag, p.err)) { ok = false; break; }
-      tc_fence_after();
       if (__any_sync(0xffffffffu, grow)) {
         const float m_new = grow ? m_blk : m_ref;
-        const float alpha = (m_ref == -INFINITY) ? 0.f : fast_exp2(m_ref - m_new);
+        const float alpha = grow ? (m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m_new)) : 1.f;
         if (i > 0) {
-#pragma unroll
+          // O is at rest once the product of the block before is complete: this block's waits for its weights
+          if (!mbar_wait(&o_full[a * 2 + (b ^ 1)], ((i - 1) >> 1) & 1, abort_flag, p.err)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll 1
           for (int cc = 0; cc < D / 16; ++cc) {
             uint32_t o16[16];
             tmem_ld_32x32b_x16(t_o + cc * 16, o16);
             tmem_ld_wait();
 #pragma unroll
-            for (int k = 0; k < 16; ++k) o16[k] = __float_as_uint(__uint_as_float(o16[k]) * (grow ? alpha : 1.f));
+            for (int k = 0; k < 16; ++k) o16[k] = __float_as_uint(__uint_as_float(o16[k]) * alpha);
             tmem_st_32x32b_x16(t_o + cc * 16, o16);
           }
         }
-        if (grow) { l *= alpha; m_ref = m_new; }
+        l *= alpha;
+        m_ref = m_new;
       }
       const float nm = C::HEAD - (m_ref == -INFINITY ? 0.f : m_ref);
       // Two forms. The FMA form of the exponential makes 2^-126 of -infinity, so it is left out where there are masked keys, which have to
       // weigh nothing even beside a sum of next to nothing. And of pages far apart in scale the one's w is nothing beside the other's,
       // its share of l is not: where a page is 2^80 below, l comes from the scores.
 #pragma unroll
-      for (int gp = 0; gp < 8; ++gp) masked |= FP8 && sc[gp].y + nm < -80.f;
+      for (int gp = 0; gp < 4; ++gp) masked |= FP8 && e[gp] + nm < -80.f;
       auto weights = [&](auto poly) {
         constexpr bool POLY = decltype(poly)::value;
 #pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
+        for (int cc = 0; cc < 2; ++cc) {
           uint32_t pk[16];
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
-            const float4 f = sc[cc * 2 + hh];
-            const float fs = fmaxf(back * f.x, 1e-37f);
-            const uint64_t f2 = f2_pack(fs, fs), n2 = f2_pack(f.y + nm, f.y + nm);
+            const int gp = cc * 2 + hh;
+            const float n1 = FP8 ? e[gp] + nm : nm;
+            const uint64_t f2 = f2_pack(fs[gp], fs[gp]), n2 = f2_pack(n1, n1);
             uint64_t sum2 = f2_pack(0.f, 0.f);
 #pragma unroll
             for (int jj = 0; jj < 8; ++jj) {
-              const int k = cc * 32 + hh * 16 + 2 * jj;
+              const int k = gp * 16 + 2 * jj;
               float y0, y1, e0, e1;
               f2_unpack(f2_fma(f2_pack_u(v[k], v[k + 1]), f2, n2), y0, y1);
-              // one pair of four on the FMA pipe, as in attention_fwd.cu
-              if (POLY && jj % 4 == 3) exp2_poly2(y0, y1, e0, e1);
+              if (POLY && PP_POLY > 0 && jj % PP_POLY == PP_POLY - 1) exp2_poly2(y0, y1, e0, e1);
               else { e0 = fast_exp2(y0); e1 = fast_exp2(y1); }
               sum2 = f2_add(sum2, f2_pack(e0, e1));
               if (FP8) {
@@ -482,25 +506,25 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
             }
             float s0, s1;
             f2_unpack(sum2, s0, s1);
-if (FP8 && !POLY) {
-              if (f.z != 0.f) {
+            if (FP8 && !POLY) {
+              if (inv[gp] != 0.f) {
 #pragma unroll
-                for (int k = cc * 32 + hh * 16; k < cc * 32 + hh * 16 + 16; ++k) l += fast_exp2(fmaf(__uint_as_float(v[k]), fs, nm));
+                for (int k = gp * 16; k < gp * 16 + 16; ++k) l += fast_exp2(fmaf(__uint_as_float(v[k]), fs[gp], nm));
               }
             } else {
-              l = FP8 ? fmaf(s0 + s1, f.z, l) : l + (s0 + s1);
+              l = FP8 ? fmaf(s0 + s1, inv[gp], l) : l + (s0 + s1);
             }
           }
-          tmem_st_32x32b_x16(t_p + cc * 16, pk);
+          tmem_st_32x32b_x16(t_s + cc * 16, pk);
         }
       };
       if (__any_sync(0xffffffffu, masked)) weights(std::false_type{});
       else weights(std::true_type{});
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[a]);
+      warp_arrive(&p_full[a * 2 + b]);
     }
-    const bool have = group && ok && nblk > 0 && mbar_wait(&o_full[a], (nblk - 1) & 1, abort_flag, p.err);
+    const bool have = ok && nblk > 0 && mbar_wait(&o_full[a * 2 + ((nblk - 1) & 1)], ((nblk - 1) >> 1) & 1, abort_flag, p.err);
     if (have) tc_fence_after();
     if (p.splits > 1) {
       const size_t at = ((static_cast<size_t>(blockIdx.z) * p.tiles + blockIdx.y) * p.Hkv + kh) * 256 + a * 128 + t;
@@ -519,10 +543,10 @@ if (FP8 && !POLY) {
             *reinterpret_cast<uint4*>(po + cc * 16 + k) = make_uint4(o16[k], o16[k + 1], o16[k + 2], o16[k + 3]);
         }
       }
-      if (live) *reinterpret_cast<float2*>(ml) = make_float2(have ? m_ref : -INFINITY, l);
+      if (live) *reinterpret_cast<float2*>(ml) = make_float2(have ? m_ref : -INFINITY, have ? l : 0.f);
     } else {
       // (a sum of nothing: no key, zeros; a NaN stays one)
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv_l = l == 0.f ? 0.f : 1.f / l;
       __nv_bfloat16* dst = p.o + (tl.row0 + row) * p.o_ld + head * p.o_head;
 #pragma unroll
       for (int cc = 0; cc < D / 16; ++cc) {
@@ -537,10 +561,10 @@ if (FP8 && !POLY) {
 #pragma unroll
           for (int k = 0; k < 16; k += 8) {
             uint4 w;
-            w.x = pack_bf16(__uint_as_float(o16[k + 0]) * inv, __uint_as_float(o16[k + 1]) * inv);
-            w.y = pack_bf16(__uint_as_float(o16[k + 2]) * inv, __uint_as_float(o16[k + 3]) * inv);
-            w.z = pack_bf16(__uint_as_float(o16[k + 4]) * inv, __uint_as_float(o16[k + 5]) * inv);
-            w.w = pack_bf16(__uint_as_float(o16[k + 6]) * inv, __uint_as_float(o16[k + 7]) * inv);
+            w.x = pack_bf16(__uint_as_float(o16[k + 0]) * inv_l, __uint_as_float(o16[k + 1]) * inv_l);
+            w.y = pack_bf16(__uint_as_float(o16[k + 2]) * inv_l, __uint_as_float(o16[k + 3]) * inv_l);
+            w.z = pack_bf16(__uint_as_float(o16[k + 4]) * inv_l, __uint_as_float(o16[k + 5]) * inv_l);
+            w.w = pack_bf16(__uint_as_float(o16[k + 6]) * inv_l, __uint_as_float(o16[k + 7]) * inv_l);
             *reinterpret_cast<uint4*>(dst + cc * 16 + k) = w;
           }
         }
