@@ -48,9 +48,6 @@ struct PagedPrefillParams {
   unsigned int* err;
 };
 
-#ifndef PP_POLY
-#define PP_POLY 8
-#endif
 constexpr int PP_THREADS = 512, PP_KEYS = 64;
 template <int D, bool FP8>
 struct PagedPrefill {
@@ -313,45 +310,57 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       }
     }
   } else if (warp >= 8) {
-    if (warp == 8 && lane == 0 && nblk > 0) {
+    // (whole warps go through these loops and one elected thread issues, so that the descriptors, the same for all, stay in uniform
+    // registers: from a lane of its own an instruction took 100 cycles to issue)
+    if (warp == 8 && nblk > 0) {
       // -------------------------------------------------------------- S = Q K^T
       constexpr uint32_t idesc = FP8 ? make_idesc_f16(128, PP_KEYS, 0, 0) : make_idesc_bf16(128, PP_KEYS, 0, 0);
-      const uint32_t q_base = smem_u32(smem), k_base = smem_u32(smem + C::OFF_K);
+      const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem), 16, 1024), k_desc = make_smem_desc_sw128(smem_u32(smem + C::OFF_K), 16, 1024);
       bool ok = mbar_wait(q_full, 0, abort_flag, p.err);
       for (int i = 0; i < nblk && ok; ++i) {
         const int ks = i % NS, b = i & 1;
-        if (!mbar_wait(&k_full[ks], (i / NS) & 1, abort_flag, p.err)) break;
+        ok = mbar_wait(&k_full[ks], (i / NS) & 1, abort_flag, p.err);
         for (int a = 0; a < tiles_here && ok; ++a) {
           // the buffer held the weights of block i - 2
           if (i > 1) ok = mbar_wait(&o_full[a * 2 + b], ((i - 2) >> 1) & 1, abort_flag, p.err);
-          if (!ok) break;
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
           tc_fence_after();
+          const uint64_t qa = q_desc + a * (C::TILE >> 4), kb = k_desc + ks * (C::KTILE >> 4);       // (addresses in 16 bytes)
+          const uint32_t to = tmem_base + a * 128 + b * 64;
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            umma_bf16(tmem_base + a * 128 + b * 64, make_smem_desc_sw128(q_base + a * C::TILE + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024),
-                      make_smem_desc_sw128(k_base + ks * C::KTILE + (kk >> 2) * (PP_KEYS * 128) + (kk & 3) * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
-          umma_commit(&s_full[a * 2 + b]);
+            for (int kk = 0; kk < D / 16; ++kk)
+              umma_bf16(to, qa + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), kb + (((kk >> 2) * (PP_KEYS * 128) + (kk & 3) * 32) >> 4), idesc,
+                        kk > 0 ? 1u : 0u);
+            umma_commit(&s_full[a * 2 + b]);
+            if (a == tiles_here - 1) umma_commit(&k_empty[ks]);
+          }
+          __syncwarp();
         }
-        if (ok) umma_commit(&k_empty[ks]);
       }
-    } else if (warp == 9 && lane == 0 && nblk > 0) {
+    } else if (warp == 9 && nblk > 0) {
       // -------------------------------------------------------------- O += P V
       constexpr uint32_t idesc = FP8 ? make_idesc_f16(128, D, 0, 1) : make_idesc_bf16(128, D, 0, 1);
-      const uint32_t v_base = smem_u32(smem + C::OFF_V);
+      const uint64_t v_desc = make_smem_desc_sw128(smem_u32(smem + C::OFF_V), PP_KEYS * 128, 1024);
       bool ok = true;
       for (int i = 0; i < nblk && ok; ++i) {
         const int vs = i % NS, b = i & 1;
-        if (!mbar_wait(&v_full[vs], (i / NS) & 1, abort_flag, p.err)) break;
+        ok = mbar_wait(&v_full[vs], (i / NS) & 1, abort_flag, p.err);
         for (int a = 0; a < tiles_here && ok; ++a) {
-          if (!mbar_wait(&p_full[a * 2 + b], (i >> 1) & 1, abort_flag, p.err)) { ok = false; break; }
+          ok = mbar_wait(&p_full[a * 2 + b], (i >> 1) & 1, abort_flag, p.err);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
           tc_fence_after();
+          const uint64_t vd = v_desc + vs * (C::KTILE >> 4);
+          const uint32_t to = tmem_base + C::COL_O + a * D, from = tmem_base + a * 128 + b * 64;
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < PP_KEYS / 16; ++kk)
-            umma_bf16_ta(tmem_base + C::COL_O + a * D, tmem_base + a * 128 + b * 64 + 8 * kk,
-                         make_smem_desc_sw128(v_base + vs * C::KTILE + kk * 2048, PP_KEYS * 128, 1024), idesc, (i > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&o_full[a * 2 + b]);
+            for (int kk = 0; kk < PP_KEYS / 16; ++kk)
+              umma_bf16_ta(to, from + 8 * kk, vd + ((kk * 2048) >> 4), idesc, (i > 0 || kk > 0) ? 1u : 0u);
+            umma_commit(&o_full[a * 2 + b]);
+            if (a == tiles_here - 1) umma_commit(&v_empty[vs]);
+          }
+          __syncwarp();
         }
-        if (ok) umma_commit(&v_empty[vs]);
       }
     }
     __syncwarp();
@@ -473,13 +482,13 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
         m_ref = m_new;
       }
       const float nm = C::HEAD - (m_ref == -INFINITY ? 0.f : m_ref);
-      // Two forms. The FMA form of the exponential makes 2^-126 of -infinity, so it is left out where there are masked keys, which have to
-      // weigh nothing even beside a sum of next to nothing. And of pages far apart in scale the one's w is nothing beside the other's,
-      // its share of l is not: where a page is 2^80 below, l comes from the scores.
+      // (of pages far apart in scale the one's w is nothing beside the other's, its share of l is not: where a page is 2^80 below, l comes
+      // from the scores)
+      bool apart = false;
 #pragma unroll
-      for (int gp = 0; gp < 4; ++gp) masked |= FP8 && e[gp] + nm < -80.f;
-      auto weights = [&](auto poly) {
-        constexpr bool POLY = decltype(poly)::value;
+      for (int gp = 0; gp < 4; ++gp) apart |= FP8 && e[gp] + nm < -80.f;
+      auto weights = [&](auto far) {
+        constexpr bool FAR = decltype(far)::value;
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
           uint32_t pk[16];
@@ -492,10 +501,9 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
 #pragma unroll
             for (int jj = 0; jj < 8; ++jj) {
               const int k = gp * 16 + 2 * jj;
-              float y0, y1, e0, e1;
+              float y0, y1;
               f2_unpack(f2_fma(f2_pack_u(v[k], v[k + 1]), f2, n2), y0, y1);
-              if (POLY && PP_POLY > 0 && jj % PP_POLY == PP_POLY - 1) exp2_poly2(y0, y1, e0, e1);
-              else { e0 = fast_exp2(y0); e1 = fast_exp2(y1); }
+              const float e0 = fast_exp2(y0), e1 = fast_exp2(y1);
               sum2 = f2_add(sum2, f2_pack(e0, e1));
               if (FP8) {
                 const __half2 h = __floats2half2_rn(e0, e1);
@@ -506,7 +514,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
             }
             float s0, s1;
             f2_unpack(sum2, s0, s1);
-            if (FP8 && !POLY) {
+            if (FAR) {
               if (inv[gp] != 0.f) {
 #pragma unroll
                 for (int k = gp * 16; k < gp * 16 + 16; ++k) l += fast_exp2(fmaf(__uint_as_float(v[k]), fs[gp], nm));
@@ -518,8 +526,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
           tmem_st_32x32b_x16(t_s + cc * 16, pk);
         }
       };
-      if (__any_sync(0xffffffffu, masked)) weights(std::false_type{});
-      else weights(std::true_type{});
+      if (FP8 && __any_sync(0xffffffffu, apart)) weights(std::integral_constant<bool, FP8>{});
+      else weights(std::false_type{});
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&p_full[a * 2 + b]);
