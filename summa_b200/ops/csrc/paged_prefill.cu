@@ -11,10 +11,12 @@
 //   warp 9            issues O += P V
 //   warps 12-15       bring keys and values from their pages into the swizzled tiles that the products read: bf16 as 16-byte
 //                     asynchronous copies, e4m3 through registers, where it becomes f16
-// A group has two score buffers of 64 columns, each with its weights in place, so the scores of the next block are computed while the
-// threads are at this one, and they wait for a product only where their maximum makes them rescale O. (With one buffer of 128 columns a
-// block took 6500 cycles, 2300 of them each group's wait for its two products.) Products of 64 columns cost 45 cycles where 128 cost 64:
-// 2464 cycles of the tensor core for 128 keys and 256 pairs instead of 2048, but it was busy a third of the time.
+// Tensor memory holds the two groups' O (256 columns), one buffer of 64 scores and two of packed weights each. The scores' buffer is free
+// again as soon as the threads have them in registers, so the scores of the next block are computed while the threads are at this one,
+// and the product with its weights while they are at the next; they wait for one only where their maximum makes them rescale O. (One
+// buffer of 128 scores with the weights in place: 6500 cycles for 128 keys, 2300 of them each group's wait for its two products. Two
+// buffers of 64, in place: 4200.) Products of 64 columns cost 48 cycles of the shared memory port where 128 cost 64: 2560 cycles for 128
+// keys and 256 pairs instead of 2048.
 // (A bulk tensor copy could fetch bf16 pages, but not expand codes, nor leave out single rows of a page that hold nothing yet: what
 // lies behind a sequence's last row may be NaN, and 0 * NaN would reach its sums.)
 //
@@ -57,7 +59,7 @@ struct PagedPrefill {
   static constexpr int RING = 8;                                 // blocks whose scales are kept: more than can be under way
   static constexpr int OFF_BAR = OFF_SCALE + RING * 4 * 16;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
-  static constexpr int COL_O = 256;                              // S (and P in place) of group a, buffer b at a * 128 + b * 64
+  static constexpr int COL_P = 128, COL_O = 256;                 // S of group a at a * 64, P at COL_P + (a * 2 + buffer) * 32, O at COL_O + a * D
   static constexpr int CPR = (FP8 ? D : 2 * D) / 16;             // 16-byte chunks of a key
   static constexpr int LOADS = PP_KEYS * CPR / 128;              // of a copying thread, per tile of 64 keys
   static constexpr float HEAD = FP8 ? 9.f : 0.f, SLACK = FP8 ? 6.f : 8.f;
@@ -123,8 +125,9 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   // (where threads arrive, a warp's have fenced what they did, and one of them does)
   uint64_t* q_full = bars + 0;    // 8 arrivals
-  uint64_t* s_full = bars + 1;    // [2 groups][2 buffers]
-  uint64_t* p_full = bars + 5;    // [2][2], 4 arrivals
+  uint64_t* s_full = bars + 1;    // [2]
+  uint64_t* s_free = bars + 3;    // [2], 4 arrivals: the group has its scores in registers
+  uint64_t* p_full = bars + 5;    // [2][2 buffers], 4 arrivals
   uint64_t* o_full = bars + 9;    // [2][2] the product with a buffer's weights is complete (one for each buffer: who waits is a phase behind at most)
   uint64_t* k_full = bars + 13;   // [NS], 4 arrivals
   uint64_t* k_empty = bars + 17;
@@ -171,7 +174,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 8);
-    for (int s = 0; s < 4; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
+    for (int s = 0; s < 4; ++s) { mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&s_full[a], 1); mbar_init(&s_free[a], 4); }
     for (int s = 0; s < NS; ++s) {
       mbar_init(&k_full[s], 4); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 4); mbar_init(&v_empty[s], 1);
     }
@@ -186,57 +190,92 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
 
   if (warp >= 12) {
     // ---------------------------------------------------------------- copies
+    // Chunk x of a thread is row x * RPI + r0 of the tile, chunk c of the row; 16 rows of one page share a look-up, done a block ahead.
     const int tid = threadIdx.x - 384, shift = p.batch.page_shift, mask = (1 << shift) - 1;
     const int* table = p.batch.table + tl.b * p.batch.table_ld;
-    // chunk i of a thread: row i * RPI + r0 of the tile, chunk c of the row
-    constexpr int RPI = 128 / C::CPR, LOADS = C::LOADS, IDS = RPI >= 16 ? LOADS : 4;   // IDS: pages that a thread meets in a tile
-    const int r0 = tid / C::CPR, c = tid % C::CPR;
-    const uint8_t *kb = p.k + kh * p.k_head + c * 16, *vb = p.v + kh * p.v_head + c * 16;
-    int id[IDS], next[IDS];
+    constexpr int ROWB = C::CPR * 16, RPI = 128 / C::CPR, LOADS = C::LOADS, IDS = RPI >= 16 ? LOADS : 4;
+    const int r0 = tid / C::CPR, c = tid % C::CPR, group0 = RPI >= 16 ? r0 & ~15 : 0;      // first row of id 0's group
+    constexpr int IDROWS = RPI >= 16 ? RPI : 16;                                           // rows between two ids' groups
+    const uint32_t lane_off = (r0 - group0) * ROWB + c * 16;
+    const uint8_t *kb = p.k + kh * p.k_head + lane_off, *vb = p.v + kh * p.v_head + lane_off;
+    const unsigned pages = p.batch.num_pages;
+    int id[IDS], next[IDS], group_next = -2;    // (group_next: of group tid, for the scales)
     auto look_up = [&](int j) {
+      group_next = -2;
+      if (tid < 4 && j < j1 && j * PP_KEYS + tid * 16 + 16 > lo && j * PP_KEYS + tid * 16 < hi) group_next = table[(j * PP_KEYS + tid * 16) >> shift];
 #pragma unroll
       for (int i = 0; i < IDS; ++i) {
-        const int key = j * PP_KEYS + (RPI >= 16 ? i * RPI + r0 : i * 16);
+        const int key = j * PP_KEYS + i * IDROWS + group0;
         next[i] = -2;
-        if (j < j1 && (key | 15) >= lo && (key & ~15) < hi) next[i] = table[key >> shift];
+        if (j < j1 && key + 16 > lo && key < hi) next[i] = table[key >> shift];
       }
     };
-    auto source = [&](const uint8_t* base, long stride, int i, int j, bool* in) -> const uint8_t* {
-      const int page = id[RPI >= 16 ? i : i * RPI / 16], key = j * PP_KEYS + i * RPI + r0;
-      *in = static_cast<unsigned>(page) < static_cast<unsigned>(p.batch.num_pages) && key >= lo && key < hi;
-      return base + (*in ? static_cast<uint64_t>(page) * static_cast<uint32_t>(stride) + static_cast<uint32_t>((key & mask) * (C::CPR * 16)) : 0);
+    // Copies of block j through take(x, source, whether it is a key of the sequence). Where all of them are, the addresses of a group are
+    // one multiplication and constants.
+    auto each = [&](const uint8_t* base, long stride, int j, auto take) {
+      bool all = j * PP_KEYS >= lo && (j + 1) * PP_KEYS <= hi;
+#pragma unroll
+      for (int i = 0; i < IDS; ++i) all = all && static_cast<unsigned>(id[i]) < pages;
+      if (all) {
+#pragma unroll
+        for (int i = 0; i < IDS; ++i) {
+          const uint8_t* src = base + (static_cast<uint64_t>(static_cast<uint32_t>(id[i])) * static_cast<uint32_t>(stride) +
+                                       static_cast<uint32_t>(((j * PP_KEYS + i * IDROWS + group0) & mask) * ROWB));
+#pragma unroll
+          for (int x = 0; x < LOADS / IDS; ++x) take(i * (LOADS / IDS) + x, src + x * RPI * ROWB, true);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < IDS; ++i) {
+          const int key = j * PP_KEYS + i * IDROWS + group0;
+          const bool good = static_cast<unsigned>(id[i]) < pages;
+          const uint8_t* src = base + (good ? static_cast<uint64_t>(static_cast<uint32_t>(id[i])) * static_cast<uint32_t>(stride) +
+                                              static_cast<uint32_t>((key & mask) * ROWB) : 0);
+#pragma unroll
+          for (int x = 0; x < LOADS / IDS; ++x) {
+            const int at = key + (r0 - group0) + x * RPI;
+            const bool in = good && at >= lo && at < hi;
+            take(i * (LOADS / IDS) + x, in ? src + x * RPI * ROWB : p.k, in);
+          }
+        }
+      }
     };
     // where elements 8 e .. 8 e + 7 of row r lie in a tile: 64 elements a row of a swizzled half
     auto place = [&](int r, int e) -> uint32_t { return (e >> 3) * (PP_KEYS * 128) + r * 128 + (((e & 7) ^ (r & 7)) << 4); };
-    // the scales of block j's groups of 16 keys, read by the softmax threads behind S
-    auto put_scales = [&](int i, int j) {
+    // The scales of a block's groups of 16 keys, read by the softmax threads behind S: asked for when its pages are known, put down with
+    // its keys. By four threads, each for a group.
+    float4 scale = make_float4(1.f, 0.f, 0.f, 0.f);
+    auto ask_scales = [&](int page) {
+      const bool good = static_cast<unsigned>(page) < pages;
+      if (!good && page != -2) atomicOr(p.err, 4u);
+      scale.z = good ? 1.f : 0.f;
+      if (FP8 && good) { scale.x = p.ks[page * p.ks_ld + kh]; scale.y = p.vs[page * p.vs_ld + kh]; }
+    };
+    auto put_scales = [&](int i) {
       if (tid < 4) {
-        const int key = j * PP_KEYS + tid * 16;
-        int page = -1;
-        if (key + 16 > lo && key < hi) {
-          page = table[key >> shift];
-          if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.batch.num_pages)) { page = -1; atomicOr(p.err, 4u); }
-        }
-        float4 f = make_float4(1.f, 0.f, page >= 0 ? 1.f : 0.f, 0.f);
-        if (FP8 && page >= 0) {
-          const int e = min(max(scale_exp(p.vs[page * p.vs_ld + kh]), PAGED_LEAST_EXP), PAGED_MOST_EXP);
-          f = make_float4(p.ks[page * p.ks_ld + kh], static_cast<float>(e), exp_scale(-e), 0.f);
+        float4 f = scale;
+        if (FP8) {
+          const int e = min(max(scale_exp(scale.y), PAGED_LEAST_EXP), PAGED_MOST_EXP);
+          f = f.z != 0.f ? make_float4(scale.x, static_cast<float>(e), exp_scale(-e), 0.f) : make_float4(1.f, 0.f, 0.f, 0.f);
         }
         scales[(i % C::RING) * 4 + tid] = f;
       }
+    };
+    auto turn = [&](int j) {                     // to block j
+#pragma unroll
+      for (int x = 0; x < IDS; ++x) id[x] = next[x];
+      if (tid < 4) ask_scales(group_next);
+      look_up(j + 1);
     };
     bool ok = true;
     look_up(j0);
     if (FP8) {
       uint4 rk[LOADS], rv[LOADS];
       auto load = [&](uint4* r, const uint8_t* base, long stride, int j) {
-#pragma unroll
-        for (int x = 0; x < LOADS; ++x) {
-          bool in;
-          const uint8_t* src = source(base, stride, x, j, &in);
-          r[x] = make_uint4(0, 0, 0, 0);
+        each(base, stride, j, [&](int x, const uint8_t* src, bool in) {
           if (in) r[x] = *reinterpret_cast<const uint4*>(src);
-        }
+          else r[x] = make_uint4(0, 0, 0, 0);
+        });
       };
       auto store = [&](const uint4* r, uint8_t* dst) {
 #pragma unroll
@@ -252,17 +291,12 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
         }
         fence_proxy_async_smem();
       };
-      auto turn = [&](int j) {
-#pragma unroll
-        for (int x = 0; x < IDS; ++x) id[x] = next[x];
-        look_up(j + 1);
-      };
       turn(j0);
       if (nblk > 0) load(rk, kb, p.k_page, j0);
       for (int i = 0; i < nblk && ok; ++i) {
         const int s = i % NS;
         load(rv, vb, p.v_page, j0 + i);
-        put_scales(i, j0 + i);
+        put_scales(i);
         ok = mbar_wait(&k_empty[s], ((i / NS) & 1) ^ 1, abort_flag, p.err);
         if (!ok) break;
         store(rk, smem + C::OFF_K + s * C::KTILE);
@@ -281,20 +315,17 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
         const int i = n >> 1, j = j0 + i, s = i % NS;
         const bool is_v = n & 1;
         if (!is_v) {
-#pragma unroll
-          for (int x = 0; x < IDS; ++x) id[x] = next[x];
-          look_up(j + 1);
-          put_scales(i, j);
+          turn(j);
+          put_scales(i);
         }
         ok = mbar_wait(is_v ? &v_empty[s] : &k_empty[s], ((i / NS) & 1) ^ 1, abort_flag, p.err);
         if (!ok) break;
         uint8_t* dst = smem + (is_v ? C::OFF_V : C::OFF_K) + s * C::KTILE;
-#pragma unroll
-        for (int x = 0; x < LOADS; ++x) {
-          bool in;
-          const uint8_t* src = source(is_v ? vb : kb, is_v ? p.v_page : p.k_page, x, j, &in);
-          cp_async16_zfill(smem_u32(dst + place(x * RPI + r0, c)), src, in ? 16 : 0);
-        }
+        const uint32_t at = smem_u32(dst) + place(r0, c);
+        each(is_v ? vb : kb, is_v ? p.v_page : p.k_page, j, [&](int x, const uint8_t* src, bool in) {
+          // (rows x * RPI: the swizzle of r0's)
+          cp_async16_zfill(at + x * RPI * 128, src, in ? 16 : 0);
+        });
         cp_async_commit();
         if (n >= 2) {
           cp_async_wait_group<2>();
@@ -318,21 +349,20 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem), 16, 1024), k_desc = make_smem_desc_sw128(smem_u32(smem + C::OFF_K), 16, 1024);
       bool ok = mbar_wait(q_full, 0, abort_flag, p.err);
       for (int i = 0; i < nblk && ok; ++i) {
-        const int ks = i % NS, b = i & 1;
+        const int ks = i % NS;
         ok = mbar_wait(&k_full[ks], (i / NS) & 1, abort_flag, p.err);
         for (int a = 0; a < tiles_here && ok; ++a) {
-          // the buffer held the weights of block i - 2
-          if (i > 1) ok = mbar_wait(&o_full[a * 2 + b], ((i - 2) >> 1) & 1, abort_flag, p.err);
+          if (i > 0) ok = mbar_wait(&s_free[a], (i - 1) & 1, abort_flag, p.err);
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
           tc_fence_after();
           const uint64_t qa = q_desc + a * (C::TILE >> 4), kb = k_desc + ks * (C::KTILE >> 4);       // (addresses in 16 bytes)
-          const uint32_t to = tmem_base + a * 128 + b * 64;
+          const uint32_t to = tmem_base + a * 64;
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
               umma_bf16(to, qa + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), kb + (((kk >> 2) * (PP_KEYS * 128) + (kk & 3) * 32) >> 4), idesc,
                         kk > 0 ? 1u : 0u);
-            umma_commit(&s_full[a * 2 + b]);
+            umma_commit(&s_full[a]);
             if (a == tiles_here - 1) umma_commit(&k_empty[ks]);
           }
           __syncwarp();
@@ -351,7 +381,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
           tc_fence_after();
           const uint64_t vd = v_desc + vs * (C::KTILE >> 4);
-          const uint32_t to = tmem_base + C::COL_O + a * D, from = tmem_base + a * 128 + b * 64;
+          const uint32_t to = tmem_base + C::COL_O + a * D, from = tmem_base + C::COL_P + (a * 2 + b) * 32;
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < PP_KEYS / 16; ++kk)
@@ -371,7 +401,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     const bool live = x < pairs;
     const int row = live ? static_cast<int>(x / p.G) : 0, head = kh * p.G + (live ? static_cast<int>(x % p.G) : 0);
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_o = tmem_base + C::COL_O + a * D + lane_sel;
+    const uint32_t t_s = tmem_base + a * 64 + lane_sel, t_o = tmem_base + C::COL_O + a * D + lane_sel;
 
     // the query row into its tile; in 8 bits as f16, scaled by a power of two
     float back = p.scale_log2;
@@ -427,8 +457,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
 #pragma unroll 1
     for (int i = 0; i < nblk && ok; ++i) {
       const int kv0 = (j0 + i) * PP_KEYS, b = i & 1;
-      const uint32_t t_s = tmem_base + a * 128 + b * 64 + lane_sel;
-      if (!mbar_wait(&s_full[a * 2 + b], (i >> 1) & 1, abort_flag, p.err)) { ok = false; break; }
+      if (!mbar_wait(&s_full[a], i & 1, abort_flag, p.err)) { ok = false; break; }
       tc_fence_after();
       uint32_t v[64];
       tmem_ld_32x32b_x32(t_s, v);
@@ -445,6 +474,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
         fs[gp] = FP8 ? fs[gp] * back : back;
       }
       tmem_ld_wait();
+      tc_fence_before();
+      warp_arrive(&s_free[a]);
       if (masked) {
         const int from = klo - kv0, to = khi - kv0;
 #pragma unroll
@@ -480,6 +511,11 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
         }
         l *= alpha;
         m_ref = m_new;
+      }
+      // this buffer's weights of two blocks ago have been used
+      if (i > 1) {
+        if (!mbar_wait(&o_full[a * 2 + b], ((i - 2) >> 1) & 1, abort_flag, p.err)) { ok = false; break; }
+        tc_fence_after();
       }
       const float nm = C::HEAD - (m_ref == -INFINITY ? 0.f : m_ref);
       // (of pages far apart in scale the one's w is nothing beside the other's, its share of l is not: where a page is 2^80 below, l comes
@@ -523,7 +559,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
               l = FP8 ? fmaf(s0 + s1, inv[gp], l) : l + (s0 + s1);
             }
           }
-          tmem_st_32x32b_x16(t_s + cc * 16, pk);
+          tmem_st_32x32b_x16(tmem_base + C::COL_P + (a * 2 + b) * 32 + lane_sel + cc * 16, pk);
         }
       };
       if (FP8 && __any_sync(0xffffffffu, apart)) weights(std::integral_constant<bool, FP8>{});
