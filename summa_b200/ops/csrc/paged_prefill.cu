@@ -5,8 +5,8 @@
 // in tensor memory. A tile is 256 (row, head) pairs of one sequence and one kv head, rows first: pair x is row x / G, query head x % G.
 // All heads that share the kv head ride in one tile, so the keys and values that it takes from the cache, and expands, serve G times
 // the rows, and a short chunk fills the tile. Two groups of 128 pairs take turns on the tensor core:
-//   warps 0-3 / 4-7   a thread per pair: its query row to shared memory, then per block of 64 keys its scores from tensor memory,
-//                     masks, running maximum, weights back into tensor memory as operand A of the next product; at the end its output row
+//   warps 0-3 / 4-7   first the query rows to shared memory; then a thread per pair: per block of 64 keys its scores from tensor memory, masks, running maximum, weights back into
+//                     tensor memory as operand A of the next product; at the end its output row, through shared memory
 //   warp 8            issues S = Q K^T
 //   warp 9            issues O += P V
 //   warps 12-15       bring keys and values from their pages into the swizzled tiles that the products read: bf16 as 16-byte
@@ -57,7 +57,8 @@ struct PagedPrefill {
   static constexpr int NS = 4;                                   // stages of keys and of values
   static constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + NS * KTILE, OFF_SCALE = OFF_V + NS * KTILE;
   static constexpr int RING = 8;                                 // blocks whose scales are kept: more than can be under way
-  static constexpr int OFF_BAR = OFF_SCALE + RING * 4 * 16;
+  static constexpr int OFF_BACK = OFF_SCALE + RING * 4 * 16;     // [256] floats: the rows' factors
+  static constexpr int OFF_BAR = OFF_BACK + 1024;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
   static constexpr int COL_P = 128, COL_O = 256;                 // S of group a at a * 64, P at COL_P + (a * 2 + buffer) * 32, O at COL_O + a * D
   static constexpr int CPR = (FP8 ? D : 2 * D) / 16;             // 16-byte chunks of a key
@@ -88,7 +89,7 @@ __device__ __forceinline__ PrefillTile prefill_tile(const PagedBatch& p, int G, 
   int front = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int rows = b0 + lane < p.B ? paged_seq(p, b0 + lane).rows : 0;
-    const int n = static_cast<int>((static_cast<long>(rows) * G + 255) / 256);
+    const int n = (static_cast<unsigned>(rows) * G + 255) / 256;
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -140,23 +141,25 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kh = blockIdx.x;
   const PrefillTile tl = prefill_tile(p.batch, p.G, blockIdx.y);
-  if (p.zero_tail) {
+  // rows behind the last sequence: thread i of n of every CTA
+  auto zero_tail = [&](int i0, int n0) {
+    if (!p.zero_tail) return;
     const int t0 = paged_tail(p.batch);
     const long n = static_cast<long>(p.batch.T - t0) * p.Hq * (D / 8);
     const long cta = blockIdx.x + static_cast<long>(gridDim.x) * (blockIdx.y + static_cast<long>(gridDim.y) * blockIdx.z);
     const long ctas = static_cast<long>(gridDim.x) * gridDim.y * gridDim.z;
-    for (long i = cta * PP_THREADS + threadIdx.x; i < n; i += ctas * PP_THREADS) {
+    for (long i = cta * n0 + i0; i < n; i += ctas * n0) {
       const long row = i / (p.Hq * (D / 8));
       const int x = static_cast<int>(i % (p.Hq * (D / 8)));
       *reinterpret_cast<uint4*>(p.o + (t0 + row) * p.o_ld + (x / (D / 8)) * p.o_head + (x % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
     }
-  }
-  if (tl.b >= p.batch.B) return;
+  };
+  if (tl.b >= p.batch.B) { zero_tail(threadIdx.x, PP_THREADS); return; }
 
   // the tile's pairs and the keys that any of them sees
-  const long pairs = static_cast<long>(tl.rows) * p.G, x0 = static_cast<long>(tl.tile) * 256;
+  const unsigned pairs = static_cast<unsigned>(tl.rows) * p.G, x0 = static_cast<unsigned>(tl.tile) * 256, G = p.G;
   const int tiles_here = pairs - x0 > 128 ? 2 : 1;               // groups that have pairs
-  const int first_row = static_cast<int>(x0 / p.G), last_row = static_cast<int>((min(pairs, x0 + 256) - 1) / p.G);
+  const int first_row = x0 / G, last_row = (min(pairs, x0 + 256) - 1) / G;
   int lo = 0, hi = tl.hi;
   if (tl.len >= 0) {
     if (p.causal) hi = static_cast<int>(min(static_cast<long>(hi), static_cast<long>(tl.len) + last_row + 1));
@@ -286,8 +289,12 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
           for (int k = 0; k < 4; ++k)
             asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
                 : "=r"(h[2 * k]), "=r"(h[2 * k + 1]) : "r"(w[k]));
-          *reinterpret_cast<uint4*>(dst + place(x * RPI + r0, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4*>(dst + place(x * RPI + r0, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+          // (where a row goes to two swizzled halves, the upper half's threads begin with the second 8 elements: the halves share banks)
+          const bool upper = 2 * c >= 8;
+          *reinterpret_cast<uint4*>(dst + place(x * RPI + r0, 2 * c + (upper ? 1 : 0))) =
+              upper ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(dst + place(x * RPI + r0, 2 * c + (upper ? 0 : 1))) =
+              upper ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]);
         }
         fence_proxy_async_smem();
       };
@@ -340,6 +347,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
         warp_arrive(full(2 * nblk - 1));
       }
     }
+    zero_tail(tid, 128);
   } else if (warp >= 8) {
     // (whole warps go through these loops and one elected thread issues, so that the descriptors, the same for all, stay in uniform
     // registers: from a lane of its own an instruction took 100 cycles to issue)
@@ -397,51 +405,55 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
   } else {
     // ---------------------------------------------------------------- softmax, a thread per pair
     const int a = warp >> 2, t = threadIdx.x & 127;
-    const long x = x0 + a * 128 + t;
+    const unsigned x = x0 + a * 128 + t;
     const bool live = x < pairs;
-    const int row = live ? static_cast<int>(x / p.G) : 0, head = kh * p.G + (live ? static_cast<int>(x % p.G) : 0);
+    const int row = live ? x / G : 0;
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem_base + a * 64 + lane_sel, t_o = tmem_base + C::COL_O + a * D + lane_sel;
 
-    // the query row into its tile; in 8 bits as f16, scaled by a power of two
-    float back = p.scale_log2;
     {
-      uint4 w[D / 8];
-      const __nv_bfloat16* src = p.q + (tl.row0 + row) * p.q_ld + head * p.q_head;
+      // The query rows into their tiles: D / 8 threads a row. In 8 bits as f16, scaled by a power of two, whose inverse goes to the row's thread.
+      float* backs = reinterpret_cast<float*>(smem + C::OFF_BACK);
+      constexpr int TPR = D / 8, RPS = 256 / TPR, STEPS = 256 / RPS;
+      uint4 w[STEPS];
+      const int c = threadIdx.x % TPR;
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
+      for (int i = 0; i < STEPS; ++i) {
+        const unsigned x = x0 + i * RPS + threadIdx.x / TPR;
         w[i] = make_uint4(0, 0, 0, 0);
-        if (live) w[i] = *reinterpret_cast<const uint4*>(src + i * 8);
+        if (x < pairs) {
+          const unsigned row = x / G, head = kh * G + x % G;
+          w[i] = *reinterpret_cast<const uint4*>(p.q + (tl.row0 + row) * p.q_ld + head * p.q_head + c * 8);
+        }
       }
-      if (FP8) {
-        float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+      for (int i = 0; i < STEPS; ++i) {
+        const int r = i * RPS + threadIdx.x / TPR;
+        if (FP8) {
+          uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+          float most = 0.f;
 #pragma unroll
           for (int k = 0; k < 4; ++k) most = fmaxf(most, fmaxf(fabsf(bf16_lo(u[k])), fabsf(bf16_hi(u[k]))));
-        }
-        int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100);
-        if (most == 0.f || !(most < INFINITY)) e = 14;
-        const float mul = exp_scale(14 - e);
-        back *= exp_scale(e - 14);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+          for (int k = TPR / 2; k > 0; k >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, k, TPR));
+          int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100);
+          if (most == 0.f || !(most < INFINITY)) e = 14;
+          const float mul = exp_scale(14 - e);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const __half2 h = __floats2half2_rn(bf16_lo(u[k]) * mul, bf16_hi(u[k]) * mul);
             u[k] = *reinterpret_cast<const uint32_t*>(&h);
           }
           w[i] = make_uint4(u[0], u[1], u[2], u[3]);
+          if (c == 0) backs[r] = exp_scale(e - 14);
         }
+        *reinterpret_cast<uint4*>(smem + (r >> 7) * C::TILE + (c >> 3) * 16384 + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = w[i];
       }
-      uint8_t* tile = smem + a * C::TILE;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(tile + (i >> 3) * 16384 + t * 128 + (((i & 7) ^ (t & 7)) << 4)) = w[i];
       fence_proxy_async_smem();
       warp_arrive(q_full);
+      if (FP8) asm volatile("bar.sync 1, 256;" ::: "memory");     // (no wait in front of it that could give up)
     }
+    const float back = FP8 ? p.scale_log2 * reinterpret_cast<const float*>(smem + C::OFF_BACK)[a * 128 + t] : p.scale_log2;
 
     // keys that this pair sees: [klo, khi)
     const long pos = static_cast<long>(tl.len) + row;
@@ -570,48 +582,67 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     }
     const bool have = ok && nblk > 0 && mbar_wait(&o_full[a * 2 + ((nblk - 1) & 1)], ((nblk - 1) >> 1) & 1, abort_flag, p.err);
     if (have) tc_fence_after();
+    // The rows leave through shared memory (the group's query tile: its products are done), so that a row's bytes are stored side by
+    // side; a warp has 32 rows of 2 D bytes there: a bf16 row, or half a row in 32 bits.
+    constexpr int CH = D / 8;                    // 16-byte chunks of those
+    uint8_t* mine = smem + a * C::TILE + (warp & 3) * (32 * D * 2);
+    const unsigned xw = x0 + a * 128 + (warp & 3) * 32;
+    auto staged = [&](int r, int c) { return reinterpret_cast<uint4*>(mine + r * (D * 2) + ((c ^ (r & (CH - 1))) << 4)); };
     if (p.splits > 1) {
-      const size_t at = ((static_cast<size_t>(blockIdx.z) * p.tiles + blockIdx.y) * p.Hkv + kh) * 256 + a * 128 + t;
-      float* po = p.part + at * D;
-      float* ml = p.part + static_cast<size_t>(p.splits) * p.tiles * p.Hkv * 256 * D + at * 2;
+      const size_t at = ((static_cast<size_t>(blockIdx.z) * p.tiles + blockIdx.y) * p.Hkv + kh) * 256 + a * 128;
+      float* ml = p.part + static_cast<size_t>(p.splits) * p.tiles * p.Hkv * 256 * D + (at + t) * 2;
+      if (live) *reinterpret_cast<float2*>(ml) = make_float2(have ? m_ref : -INFINITY, have ? l : 0.f);
+      if (__all_sync(0xffffffffu, have)) {       // (what has no keys is not read again)
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int cc = 0; cc < D / 16; ++cc) {
-        uint32_t o16[16];
-        if (have) {
-          tmem_ld_32x32b_x16(t_o + cc * 16, o16);
-          tmem_ld_wait();
-        }
-        if (live && have) {
+          for (int cc = 0; cc < D / 32; ++cc) {
+            uint32_t o16[16];
+            tmem_ld_32x32b_x16(t_o + h * (D / 2) + cc * 16, o16);
+            tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < 16; k += 4)
-            *reinterpret_cast<uint4*>(po + cc * 16 + k) = make_uint4(o16[k], o16[k + 1], o16[k + 2], o16[k + 3]);
+            for (int k = 0; k < 4; ++k) *staged(lane, cc * 4 + k) = make_uint4(o16[4 * k], o16[4 * k + 1], o16[4 * k + 2], o16[4 * k + 3]);
+          }
+          __syncwarp();
+#pragma unroll 4
+          for (int i = 0; i < CH; ++i) {
+            const int r = i * (32 / CH) + lane / CH, c = lane % CH;
+            if (xw + r < pairs)
+              *reinterpret_cast<uint4*>(p.part + (at + (warp & 3) * 32 + r) * D + h * (D / 2) + c * 4) = *staged(r, c);
+          }
+          __syncwarp();
         }
       }
-      if (live) *reinterpret_cast<float2*>(ml) = make_float2(have ? m_ref : -INFINITY, have ? l : 0.f);
     } else {
       // (a sum of nothing: no key, zeros; a NaN stays one)
       const float inv_l = l == 0.f ? 0.f : 1.f / l;
-      __nv_bfloat16* dst = p.o + (tl.row0 + row) * p.o_ld + head * p.o_head;
 #pragma unroll
       for (int cc = 0; cc < D / 16; ++cc) {
         uint32_t o16[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) o16[k] = 0u;
-        if (have) {
+        if (__all_sync(0xffffffffu, have)) {
           tmem_ld_32x32b_x16(t_o + cc * 16, o16);
           tmem_ld_wait();
-        }
-        if (live) {
+        } else {
 #pragma unroll
-          for (int k = 0; k < 16; k += 8) {
-            uint4 w;
-            w.x = pack_bf16(__uint_as_float(o16[k + 0]) * inv_l, __uint_as_float(o16[k + 1]) * inv_l);
-            w.y = pack_bf16(__uint_as_float(o16[k + 2]) * inv_l, __uint_as_float(o16[k + 3]) * inv_l);
-            w.z = pack_bf16(__uint_as_float(o16[k + 4]) * inv_l, __uint_as_float(o16[k + 5]) * inv_l);
-            w.w = pack_bf16(__uint_as_float(o16[k + 6]) * inv_l, __uint_as_float(o16[k + 7]) * inv_l);
-            *reinterpret_cast<uint4*>(dst + cc * 16 + k) = w;
-          }
+          for (int k = 0; k < 16; ++k) o16[k] = 0u;
         }
+#pragma unroll
+        for (int k = 0; k < 16; k += 8) {
+          uint4 w;
+          w.x = pack_bf16(__uint_as_float(o16[k + 0]) * inv_l, __uint_as_float(o16[k + 1]) * inv_l);
+          w.y = pack_bf16(__uint_as_float(o16[k + 2]) * inv_l, __uint_as_float(o16[k + 3]) * inv_l);
+          w.z = pack_bf16(__uint_as_float(o16[k + 4]) * inv_l, __uint_as_float(o16[k + 5]) * inv_l);
+          w.w = pack_bf16(__uint_as_float(o16[k + 6]) * inv_l, __uint_as_float(o16[k + 7]) * inv_l);
+          *staged(lane, cc * 2 + k / 8) = w;
+        }
+      }
+      __syncwarp();
+#pragma unroll 4
+      for (int i = 0; i < CH; ++i) {
+        const int r = i * (32 / CH) + lane / CH, c = lane % CH;
+        const unsigned y = xw + r;
+        if (y < pairs)
+          *reinterpret_cast<uint4*>(p.o + (tl.row0 + y / G) * p.o_ld + (kh * G + y % G) * p.o_head + c * 8) = *staged(r, c);
       }
     }
   }
@@ -633,10 +664,10 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PagedPref
   const PrefillTile tl = prefill_tile(p.batch, p.G, blockIdx.y);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (tl.b >= p.batch.B) return;
-  const long pairs = static_cast<long>(tl.rows) * p.G, x0 = static_cast<long>(tl.tile) * 256;
+  const unsigned pairs = static_cast<unsigned>(tl.rows) * p.G, x0 = static_cast<unsigned>(tl.tile) * 256, G = p.G;
   const size_t stride = static_cast<size_t>(p.tiles) * p.Hkv * 256;                 // pairs between two splits
   const float* ml0 = p.part + p.splits * stride * D;
-  for (int r = blockIdx.z * 8 + warp; r < 256 && x0 + r < pairs; r += 8 * gridDim.z) {
+  for (unsigned r = blockIdx.z * 8 + warp; r < 256 && x0 + r < pairs; r += 8 * gridDim.z) {
     const size_t at = (static_cast<size_t>(blockIdx.y) * p.Hkv + kh) * 256 + r;
     float top = -INFINITY, sum = 0.f, o[V] = {};
     for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml0[(s * stride + at) * 2]);
@@ -655,7 +686,7 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PagedPref
       }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    __nv_bfloat16* dst = p.o + (tl.row0 + (x0 + r) / p.G) * p.o_ld + (kh * p.G + (x0 + r) % p.G) * p.o_head + lane * V;
+    __nv_bfloat16* dst = p.o + (tl.row0 + (x0 + r) / G) * p.o_ld + (kh * G + (x0 + r) % G) * p.o_head + lane * V;
     if (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2 % V] * inv, o[3 % V] * inv));
     else *reinterpret_cast<uint32_t*>(dst) = pack_bf16(o[0] * inv, o[1] * inv);
   }
@@ -725,7 +756,7 @@ extern "C" int sb_paged_prefill(const void* q, const void* kp, const void* vp, c
   using namespace sb;
   const int shift = page_shift_of(page);
   SB_CHECK_ARG((D == 64 || D == 128) && shift >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && T > 0 && B > 0 && P > 0 && num_pages > 0);
-  SB_CHECK_ARG((starts != nullptr || T == B) && (ks == nullptr) == (vs == nullptr) && scale > 0.f);
+  SB_CHECK_ARG((starts != nullptr || T == B) && (ks == nullptr) == (vs == nullptr) && scale > 0.f && static_cast<long>(T) * Hq < (1L << 31) - 256);
   const bool fp8 = ks != nullptr;
   const long size = fp8 ? 1 : 2;
   SB_CHECK_ARG(k_page >= 0 && v_page >= 0 && k_head >= 0 && v_head >= 0 && k_page * size < (1L << 32) && v_page * size < (1L << 32));
