@@ -169,10 +169,11 @@ def paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv: PagedKV, 
     nothing and return zeros; rows behind the last sequence are zeros, or as they were in `out`. No two sequences of a call may append
     to one page. A position without a page (or beyond cos / sin) stores nothing and returns zeros on CUDA, and sets bit 4 of the device's error
     word (`native.read_error_flag`); on the CPU it raises. No gradients."""
-    paged.check_append(qkv, q_gamma, k_gamma, cos, sin, Hq, Hkv, D, kv, rows, out)
-    _no_gradient("paged_append", qkv, q_gamma, k_gamma)
+    layout = paged.check_append(qkv, q_gamma, k_gamma, cos, sin, Hq, Hkv, D, kv, rows, out)
+    if torch.is_grad_enabled():
+        _no_gradient("paged_append", qkv, q_gamma, k_gamma)
     if native_enabled(qkv) and D in (64, 128):
-        return _cu().paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv, rows, out)
+        return _cu().paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv, rows, layout, out)
     return paged.append_reference(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv, rows, out)
 
 
@@ -183,15 +184,16 @@ def paged_attention(q, kv: PagedKV, rows: PagedRows, causal=True, window=None, s
     zeros, rows behind the last sequence zeros, or as they were in `out`. Keys without a page are left out on CUDA, and set bit 4 of the
     device's error word; on the CPU they raise. A value that is not finite reaches the rows whose sequence holds it, and no others; within
     the rows of one call it may also reach those that the mask keeps from it. No gradients."""
-    paged.check_attention(q, kv, rows, window, scale, out)
-    _no_gradient("paged_attention", q)
+    layout = paged.check_attention(q, kv, rows, window, scale, out)
+    if torch.is_grad_enabled():
+        _no_gradient("paged_attention", q)
     if native_enabled(q) and q.shape[2] in (64, 128):
-        return _cu().paged_attention(q, kv, rows, causal, window, scale, out)
+        return _cu().paged_attention(q, kv, rows, layout, causal, window, scale, out)
     return paged.attention_reference(q, kv, rows, causal, window, scale, out)
 
 
 def _no_gradient(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
 
 

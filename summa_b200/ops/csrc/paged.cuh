@@ -53,6 +53,28 @@ __device__ __forceinline__ int paged_tail(const PagedBatch& p) {
   return p.starts == nullptr ? p.T : min(max(p.starts[p.B], 0), p.T);
 }
 
+// The sequence of row t: the last one that starts at or before it. The groups of N lanes of a warp ask together, each for its own
+// row; a step of the search looks at 32 places at once.
+template <int N>
+__device__ __forceinline__ int paged_row_seq(const PagedBatch& p, int t) {
+  const int lane = threadIdx.x & 31;
+  int mine = 0;
+#pragma unroll
+  for (int g = 0; g < 32; g += N) {
+    const int row = __shfl_sync(0xffffffffu, t, g);
+    int lo = 0, n = p.B;
+    while (n > 1) {
+      const int step = (n + 31) / 32;
+      const bool before = lane * step < n && p.starts[lo + lane * step] <= row;
+      const int hit = max(__popc(__ballot_sync(0xffffffffu, before)) - 1, 0) * step;
+      lo += hit;
+      n = min(n - hit, step);
+    }
+    if (lane / N == g / N) mine = lo;
+  }
+  return mine;
+}
+
 // Page of position `pos` (>= 0) of sequence b, -1 if there is none.
 __device__ __forceinline__ int paged_page(const PagedBatch& p, int b, long pos) {
   const long i = pos >> p.page_shift;
@@ -81,6 +103,40 @@ __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t v) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v), __NV_E4M3);
   return __half22float2(__half2(h));
 }
+
+// The arguments of the C entry points, in the layout that the caller packs (no padding: 8-byte fields first, an even number of
+// 4-byte ones behind). Strides are in elements.
+struct PagedAppendArgs {
+  cudaStream_t stream;
+  const void* qkv;                   // bf16 [T, (Hq + 2 Hkv) D], row stride ld
+  void* q;                           // bf16 [T, Hq, D], row stride q_ld
+  const float *q_gamma, *k_gamma;    // [D], null: no norm
+  const float *cos, *sin;            // [max_pos, D / 2], null: no rotation
+  void *k, *v;                       // [num_pages, Hkv, page, D]: bf16, or e4m3 with scales; rows of D lie together
+  float *k_scale, *v_scale;          // [num_pages, Hkv]
+  const int *table, *lengths, *starts;   // [B, P], [B], [B + 1] or null (row b is sequence b's)
+  long ld, q_ld, table_ld, k_page, k_head, v_page, v_head, k_scale_ld, v_scale_ld;
+  int T, B, P, Hq, Hkv, D, page, num_pages, max_pos;
+  int max_rows;                      // the most rows of one sequence
+  int zero_tail;                     // rows behind the last sequence: 1 zeros, 0 left as they are
+  float eps;
+};
+struct PagedAttentionArgs {
+  cudaStream_t stream;
+  const void* q;                     // bf16 [T, Hq, D]
+  const void *k, *v;
+  const float *k_scale, *v_scale;
+  void* o;                           // as q
+  float* work;                       // as many floats as the workspace function says, null for none
+  const int *table, *lengths, *starts;
+  long q_ld, q_head, o_ld, o_head, table_ld, k_page, k_head, v_page, v_head, k_scale_ld, v_scale_ld;
+  int T, B, P, Hq, Hkv, D, page, num_pages, max_rows;
+  int causal, window;                // window < 0: none
+  int zero_tail;
+  float scale;
+  int pad;
+};
+static_assert(sizeof(PagedAppendArgs) == 14 * 8 + 9 * 8 + 12 * 4 && sizeof(PagedAttentionArgs) == 11 * 8 + 11 * 8 + 14 * 4, "packed by the caller");
 
 // Host: log2 of a page size, -1 if it is not one that the kernels take.
 inline int page_shift_of(int page) {

@@ -17,6 +17,9 @@
 
 namespace sb {
 
+constexpr int HEADS = 4;            // heads that a group of threads takes where there are many rows
+constexpr long MANY_BLOCKS = 148 * 8;    // blocks of one head, beyond which it does
+
 struct AppendParams {
   PagedBatch batch;
   const __nv_bfloat16* qkv;
@@ -44,9 +47,19 @@ __device__ __forceinline__ uint4 pack8(const float* v) {
   return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
 }
 
+// Cosines and sines of a position for the 4 pairs from `part * 4` on.
+template <int D>
+__device__ __forceinline__ void turns(const AppendParams& p, long pos, int part, float* c, float* s) {
+  if (p.cos_t == nullptr) return;
+  const float4 a = *reinterpret_cast<const float4*>(p.cos_t + pos * (D / 2) + part * 4);
+  const float4 b = *reinterpret_cast<const float4*>(p.sin_t + pos * (D / 2) + part * 4);
+  c[0] = a.x; c[1] = a.y; c[2] = a.z; c[3] = a.w;
+  s[0] = b.x; s[1] = b.y; s[2] = b.z; s[3] = b.w;
+}
+
 // Norm and rotation of the 8 elements from `part * 8` of a head; the head's other elements are in the D / 8 lanes of the group.
 template <int D>
-__device__ __forceinline__ void norm_rotate(float* v, const AppendParams& p, const float* gamma, long pos, int part) {
+__device__ __forceinline__ void norm_rotate(float* v, const AppendParams& p, const float* gamma, int part, const float* c, const float* s) {
   if (gamma != nullptr) {
     float ss = 0.f;
 #pragma unroll
@@ -59,14 +72,11 @@ __device__ __forceinline__ void norm_rotate(float* v, const AppendParams& p, con
     v[4] *= r * g1.x; v[5] *= r * g1.y; v[6] *= r * g1.z; v[7] *= r * g1.w;
   }
   if (p.cos_t != nullptr) {
-    const float4 c = *reinterpret_cast<const float4*>(p.cos_t + pos * (D / 2) + part * 4);
-    const float4 s = *reinterpret_cast<const float4*>(p.sin_t + pos * (D / 2) + part * 4);
-    const float cc[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float a = v[2 * i], b = v[2 * i + 1];
-      v[2 * i] = a * cc[i] - b * sn[i];
-      v[2 * i + 1] = a * sn[i] + b * cc[i];
+      v[2 * i] = a * c[i] - b * s[i];
+      v[2 * i + 1] = a * s[i] + b * c[i];
     }
   }
 }
@@ -115,100 +125,105 @@ __device__ __forceinline__ int grown_exp(float old, int slot, float most, float*
 }
 
 // ---------------------------------------------------------------- rows
-template <int D, bool FP8>
-__global__ void __launch_bounds__(256) paged_append_rows_kernel(const AppendParams p) {
+// Rows from blockIdx `bx` * 256 / (D / 8) on, one per group, and the heads from h0 on that lie below `heads`, HPT at most. The
+// projection's rows are asked for before anything is known of their sequence: their addresses need nothing but the row's number.
+template <int D, bool FP8, int HPT>
+__device__ __forceinline__ void append_rows(const AppendParams& p, int bx, int h0, int heads) {
   constexpr int TPH = D / 8;
-  asm volatile("griddepcontrol.launch_dependents;");
-  const int heads = p.Hq + 2 * p.Hkv;
-  const long item = (blockIdx.x * 256L + threadIdx.x) / TPH;
   const int part = threadIdx.x % TPH;
-  const bool there = item < static_cast<long>(p.batch.T) * heads;
-  const int t = there ? static_cast<int>(item / heads) : 0, h = there ? static_cast<int>(item % heads) : 0;
-  // the row's sequence: the last one that starts at or before it
-  int b = t;
-  const bool tail = t >= paged_tail(p.batch);
-  if (p.batch.starts != nullptr) {
-    int lo = 0, hi = p.batch.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (p.batch.starts[mid] <= t) lo = mid; else hi = mid - 1;
-    }
-    b = lo;
-  }
+  const long row = bx * static_cast<long>(256 / TPH) + threadIdx.x / TPH;
+  const bool there = row < p.batch.T;
+  const int t = there ? static_cast<int>(row) : p.batch.T - 1;
+  uint4 w[HPT];
+#pragma unroll
+  for (int i = 0; i < HPT; ++i)
+    if (h0 + i < heads) w[i] = *reinterpret_cast<const uint4*>(p.qkv + t * p.ld + static_cast<long>(h0 + i) * D + part * 8);
+  const int b = p.batch.starts != nullptr ? paged_row_seq<TPH>(p.batch, t) : t;
   const PagedSeq s = paged_seq(p.batch, b);
-  const bool mine = there && !tail && t >= s.row0 && t < s.row0 + s.rows;
+  const bool mine = there && t < paged_tail(p.batch) && t >= s.row0 && t < s.row0 + s.rows;
   long pos = 0;
   int page = -1;
   if (mine && s.len >= 0) {
     pos = static_cast<long>(s.len) + (t - s.row0);
     page = pos < p.max_pos ? paged_page(p.batch, b, pos) : -1;
-    if (page < 0 && h == 0 && part == 0) atomicOr(p.err, 4u);
+    if (page < 0 && h0 == 0 && part == 0) atomicOr(p.err, 4u);
   }
   const bool live = page >= 0;
-  float v[8];
-  uint4 w = make_uint4(0, 0, 0, 0);
-  if (live) w = *reinterpret_cast<const uint4*>(p.qkv + t * p.ld + static_cast<long>(h) * D + part * 8);
-  unpack8(w, v);
-  const bool is_v = h >= p.Hq + p.Hkv;
-  // (every lane of the warp takes part in the group sums; what a lane of no item computes goes nowhere)
-  float u[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) u[i] = v[i];
-  norm_rotate<D>(u, p, h < p.Hq ? p.q_gamma : p.k_gamma, pos, part);
-  if (!is_v) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = u[i];
-  }
-  if (h < p.Hq) {
-    if (there && (mine || p.zero_tail))
-      *reinterpret_cast<uint4*>(p.q + t * p.q_ld + static_cast<long>(h) * D + part * 8) = live ? pack8(v) : make_uint4(0, 0, 0, 0);
-    if (!FP8) return;
-  }
-  const int hk = is_v ? h - p.Hq - p.Hkv : h - p.Hq;
   const int slot = static_cast<int>(pos & ((1 << p.batch.page_shift) - 1));
-  if (!FP8) {
-    if (live) {
-      __nv_bfloat16* dst = is_v ? static_cast<__nv_bfloat16*>(p.vp) + page * p.v_page + hk * p.v_head
-                                : static_cast<__nv_bfloat16*>(p.kp) + page * p.k_page + hk * p.k_head;
-      *reinterpret_cast<uint4*>(dst + static_cast<long>(slot) * D + part * 8) = is_v ? w : pack8(v);
-    }
-    return;
-  }
-  float most = finite_max(v);
+  float c[4], sn[4];
+  turns<D>(p, live ? pos : 0, part, c, sn);
 #pragma unroll
-  for (int o = TPH / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o, TPH));
-  const bool put = live && h >= p.Hq;
-  float* sp = put ? (is_v ? p.vs + page * p.vs_ld + hk : p.ks + page * p.ks_ld + hk) : nullptr;
-  float ratio = 1.f;
-  int e = 0;
-  if (put) e = grown_exp(slot > 0 ? *sp : 0.f, slot, most, &ratio);
-  __syncwarp();                                        // every lane has read the old scale
-  if (!put) return;
-  uint8_t* dst = is_v ? static_cast<uint8_t*>(p.vp) + page * p.v_page + hk * p.v_head
-                      : static_cast<uint8_t*>(p.kp) + page * p.k_page + hk * p.k_head;
-  if (ratio != 1.f) move_codes(dst, slot * D, ratio, part, TPH);
-  if (part == 0) *sp = exp_scale(e);
-  *reinterpret_cast<uint2*>(dst + static_cast<long>(slot) * D + part * 8) = encode8(v, exp_scale(-e));
+  for (int i = 0; i < HPT; ++i) {
+    const int h = h0 + i;
+    if (h >= heads) return;
+    const bool is_v = h >= p.Hq + p.Hkv;
+    float v[8];
+    unpack8(w[i], v);
+    if (!is_v) norm_rotate<D>(v, p, h < p.Hq ? p.q_gamma : p.k_gamma, part, c, sn);
+    if (h < p.Hq) {
+      if (there && (mine || p.zero_tail))
+        *reinterpret_cast<uint4*>(p.q + t * p.q_ld + static_cast<long>(h) * D + part * 8) = live ? pack8(v) : make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const int hk = is_v ? h - p.Hq - p.Hkv : h - p.Hq;
+    if (!FP8) {
+      if (live) {
+        __nv_bfloat16* dst = is_v ? static_cast<__nv_bfloat16*>(p.vp) + page * p.v_page + hk * p.v_head
+                                  : static_cast<__nv_bfloat16*>(p.kp) + page * p.k_page + hk * p.k_head;
+        *reinterpret_cast<uint4*>(dst + static_cast<long>(slot) * D + part * 8) = is_v ? w[i] : pack8(v);
+      }
+      continue;
+    }
+    float most = finite_max(v);
+#pragma unroll
+    for (int o = TPH / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o, TPH));
+    float* sp = !live ? nullptr : is_v ? p.vs + page * p.vs_ld + hk : p.ks + page * p.ks_ld + hk;
+    float ratio = 1.f;
+    int e = 0;
+    if (live) e = grown_exp(slot > 0 ? *sp : 0.f, slot, most, &ratio);
+    __syncwarp();                                        // every lane has read the old scale
+    if (live) {
+      uint8_t* dst = is_v ? static_cast<uint8_t*>(p.vp) + page * p.v_page + hk * p.v_head
+                          : static_cast<uint8_t*>(p.kp) + page * p.k_page + hk * p.k_head;
+      if (ratio != 1.f) move_codes(dst, slot * D, ratio, part, TPH);
+      if (part == 0) *sp = exp_scale(e);
+      *reinterpret_cast<uint2*>(dst + static_cast<long>(slot) * D + part * 8) = encode8(v, exp_scale(-e));
+    }
+  }
+}
+
+template <int D, bool FP8, int HPT>
+__global__ void __launch_bounds__(256) paged_append_rows_kernel(const AppendParams p) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  append_rows<D, FP8, HPT>(p, blockIdx.x, blockIdx.y * HPT, p.Hq + 2 * p.Hkv);
 }
 
 // ---------------------------------------------------------------- segments
-// Block (x, y): the x-th (sequence, page) that gets rows, head y of the Hq + 2 Hkv. NP passes of 256 threads cover a page.
+// The first `q_blocks` blocks take the queries as above. Of the others, 2 Hkv per (sequence, page) that gets rows, one for each head
+// of keys and of values; NP passes of 256 threads cover the
+// rows that one of them can get, of a page or of max_rows.
 template <int D, int NP>
-__global__ void __launch_bounds__(256) paged_append_segments_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(256, NP > 4 ? 2 : 4) paged_append_segments_kernel(const AppendParams p, const int q_blocks) {
   constexpr int TPH = D / 8, RPP = 256 / TPH;        // threads of a row, rows of a pass
   __shared__ float red[8];
   asm volatile("griddepcontrol.launch_dependents;");
+  const int groups = (p.Hq + HEADS - 1) / HEADS;
+  if (static_cast<int>(blockIdx.x) < q_blocks) {
+    append_rows<D, false, HEADS>(p, blockIdx.x / groups, static_cast<int>(blockIdx.x % groups) * HEADS, p.Hq);
+    return;
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int shift = p.batch.page_shift, page_rows = 1 << shift;
+  const int shift = p.batch.page_shift;
+  int seg = (blockIdx.x - q_blocks) / (2 * p.Hkv), b = -1;
+  const int h = (blockIdx.x - q_blocks) % (2 * p.Hkv);
   // every warp finds the segment by itself: segments of 32 sequences at a time, summed over the lanes
-  int seg = blockIdx.x, b = -1;
+  PagedSeq s;
   for (int b0 = 0; b0 < p.batch.B && b < 0; b0 += 32) {
     int n = 0;
+    s = PagedSeq{0, 0, -1};
     if (b0 + lane < p.batch.B) {
-      const PagedSeq s = paged_seq(p.batch, b0 + lane);
-      // (a slot that is not in use has its rows zeroed, a page's worth at a time, as if it began at position 0)
-      const long first = max(s.len, 0);
-      if (s.rows > 0) n = static_cast<int>(((first + s.rows - 1) >> shift) - (first >> shift)) + 1;
+      s = paged_seq(p.batch, b0 + lane);
+      if (s.rows > 0 && s.len >= 0) n = static_cast<int>(((static_cast<long>(s.len) + s.rows - 1) >> shift) - (s.len >> shift)) + 1;
     }
     int sum = n;
 #pragma unroll
@@ -221,59 +236,48 @@ __global__ void __launch_bounds__(256) paged_append_segments_kernel(const Append
       const int l = __popc(__ballot_sync(0xffffffffu, sum <= seg));      // the first lane whose sum passes it
       b = b0 + l;
       seg -= __shfl_sync(0xffffffffu, sum - n, l);
+      s = PagedSeq{__shfl_sync(0xffffffffu, s.row0, l), __shfl_sync(0xffffffffu, s.rows, l), __shfl_sync(0xffffffffu, s.len, l)};
     } else {
       seg -= all;
     }
   }
-  const int h = blockIdx.y;
-  if (b < 0) {
-    // behind the last segment: rows of no sequence, a page's worth per block
-    const long t0 = paged_tail(p.batch) + static_cast<long>(seg) * page_rows;
-    if (p.zero_tail && h < p.Hq)
-      for (int r = threadIdx.x / TPH; r < page_rows && t0 + r < p.batch.T; r += RPP)
-        *reinterpret_cast<uint4*>(p.q + (t0 + r) * p.q_ld + static_cast<long>(h) * D + (threadIdx.x % TPH) * 8) = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  const PagedSeq s = paged_seq(p.batch, b);
-  const long first = max(s.len, 0);
-  const long page_no = (first >> shift) + seg, pos0 = max(first, page_no << shift);
+  if (b < 0) return;
+  const long first = s.len, page_no = (first >> shift) + seg, pos0 = max(first, page_no << shift);
   const int slot0 = static_cast<int>(pos0 - (page_no << shift));
   const int n = static_cast<int>(min(first + s.rows, (page_no + 1) << shift) - pos0);
   const long row0 = s.row0 + (pos0 - first);
-  int page = -1, live = 0;                             // rows of the segment that have a place: a page, and a row of the tables
-  if (s.len >= 0) {
-    page = paged_page(p.batch, b, pos0);
-    live = page < 0 ? 0 : static_cast<int>(min(static_cast<long>(n), max(p.max_pos - pos0, 0L)));
-    if (live < n && h == 0 && threadIdx.x == 0) atomicOr(p.err, 4u);
-  }
-  const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.Hkv;
-  const float* gamma = is_q ? p.q_gamma : is_v ? nullptr : p.k_gamma;
-  const int part = threadIdx.x % TPH;
-  float v[NP][8], most = 0.f;
+  const bool is_v = h >= p.Hkv;
+  const int part = threadIdx.x % TPH, hk = is_v ? h - p.Hkv : h;
   uint4 w[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int r = i * RPP + threadIdx.x / TPH;
-    w[i] = r < live ? *reinterpret_cast<const uint4*>(p.qkv + (row0 + r) * p.ld + static_cast<long>(h) * D + part * 8) : make_uint4(0, 0, 0, 0);
+    w[i] = r < n ? *reinterpret_cast<const uint4*>(p.qkv + (row0 + r) * p.ld + static_cast<long>(p.Hq + h) * D + part * 8) : make_uint4(0, 0, 0, 0);
   }
+  const int page = paged_page(p.batch, b, pos0);
+  // rows of the segment that have a place: a page, and a row of the tables (the queries' blocks report those that have none)
+  int live = page < 0 ? 0 : static_cast<int>(min(static_cast<long>(n), max(p.max_pos - pos0, 0L)));
+  if (live > NP * RPP) {                               // more rows than max_rows says
+    live = NP * RPP;
+    if (threadIdx.x == 0) atomicOr(p.err, 4u);
+  }
+  if (live == 0) return;
+  float* sp = is_v ? p.vs + page * p.vs_ld + hk : p.ks + page * p.ks_ld + hk;
+  const float old = slot0 > 0 ? *sp : 0.f;
+  float v[NP][8], most = 0.f;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int r = i * RPP + threadIdx.x / TPH;
     unpack8(w[i], v[i]);
-    if (!is_v) norm_rotate<D>(v[i], p, gamma, r < live ? pos0 + r : 0, part);
-    if (is_q) {
-      if (r < n)
-        *reinterpret_cast<uint4*>(p.q + (row0 + r) * p.q_ld + static_cast<long>(h) * D + part * 8) = r < live ? pack8(v[i]) : make_uint4(0, 0, 0, 0);
-    } else if (r < live) {
-      most = fmaxf(most, finite_max(v[i]));
+    if (!is_v) {
+      float c[4], sn[4];
+      turns<D>(p, r < live ? pos0 + r : 0, part, c, sn);
+      norm_rotate<D>(v[i], p, p.k_gamma, part, c, sn);
     }
+    if (r < live) most = fmaxf(most, finite_max(v[i]));
   }
-  if (is_q || live == 0) return;
   most = warp_max(most);
   if (lane == 0) red[warp] = most;
-  const int hk = is_v ? h - p.Hq - p.Hkv : h - p.Hq;
-  float* sp = is_v ? p.vs + page * p.vs_ld + hk : p.ks + page * p.ks_ld + hk;
-  const float old = slot0 > 0 ? *sp : 0.f;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) most = fmaxf(most, red[i]);
@@ -293,23 +297,31 @@ __global__ void __launch_bounds__(256) paged_append_segments_kernel(const Append
 
 template <int D>
 static int launch_append(const AppendParams& p, bool one_row, cudaStream_t st) {
+  constexpr int RPB = 256 / (D / 8);
   const int heads = p.Hq + 2 * p.Hkv;
+  const long rows = (static_cast<long>(p.batch.T) + RPB - 1) / RPB;
   if (p.ks == nullptr || one_row) {
-    const long blocks = (static_cast<long>(p.batch.T) * heads * (D / 8) + 255) / 256;
-    SB_CHECK_ARG(blocks <= 0x7fffffffL);
-    if (p.ks == nullptr) paged_append_rows_kernel<D, false><<<static_cast<int>(blocks), 256, 0, st>>>(p);
-    else paged_append_rows_kernel<D, true><<<static_cast<int>(blocks), 256, 0, st>>>(p);
+    const bool many = rows * heads > MANY_BLOCKS;
+    const dim3 grid(static_cast<unsigned>(rows), many ? (heads + HEADS - 1) / HEADS : heads);
+    SB_CHECK_ARG(grid.y <= 65535);
+    if (p.ks == nullptr) {
+      if (many) paged_append_rows_kernel<D, false, HEADS><<<grid, 256, 0, st>>>(p);
+      else paged_append_rows_kernel<D, false, 1><<<grid, 256, 0, st>>>(p);
+    } else {
+      if (many) paged_append_rows_kernel<D, true, HEADS><<<grid, 256, 0, st>>>(p);
+      else paged_append_rows_kernel<D, true, 1><<<grid, 256, 0, st>>>(p);
+    }
   } else {
-    // Rows r of a sequence touch at most (r - 1) / page + 2 pages, the rows behind the last sequence rows / page + 1 blocks.
+    // Rows r of a sequence touch at most (r - 1) / page + 2 pages.
     const int page = 1 << p.batch.page_shift;
-    const long blocks = p.batch.T / page + 2L * p.batch.B + 1;
-    SB_CHECK_ARG(blocks <= 0x7fffffffL && heads <= 65535);
-    const dim3 grid(static_cast<unsigned>(blocks), heads);
-    const int np = page * (D / 8) / 256;
-    if (np <= 1) paged_append_segments_kernel<D, 1><<<grid, 256, 0, st>>>(p);
-    else if (np == 2) paged_append_segments_kernel<D, 2><<<grid, 256, 0, st>>>(p);
-    else if (np == 4) paged_append_segments_kernel<D, 4><<<grid, 256, 0, st>>>(p);
-    else paged_append_segments_kernel<D, 8><<<grid, 256, 0, st>>>(p);
+    const long q_blocks = rows * ((p.Hq + HEADS - 1) / HEADS), blocks = q_blocks + (p.batch.T / page + 2L * p.batch.B) * 2 * p.Hkv;
+    SB_CHECK_ARG(blocks <= 0x7fffffffL);
+    const unsigned grid = static_cast<unsigned>(blocks);
+    const int np = (min(page, p.batch.max_rows) + RPB - 1) / RPB;
+    if (np <= 1) paged_append_segments_kernel<D, 1><<<grid, 256, 0, st>>>(p, static_cast<int>(q_blocks));
+    else if (np == 2) paged_append_segments_kernel<D, 2><<<grid, 256, 0, st>>>(p, static_cast<int>(q_blocks));
+    else if (np <= 4) paged_append_segments_kernel<D, 4><<<grid, 256, 0, st>>>(p, static_cast<int>(q_blocks));
+    else paged_append_segments_kernel<D, 8><<<grid, 256, 0, st>>>(p, static_cast<int>(q_blocks));
   }
   SB_CHECK_CUDA(cudaGetLastError());
   return SB_OK;
@@ -317,30 +329,26 @@ static int launch_append(const AppendParams& p, bool one_row, cudaStream_t st) {
 
 }  // namespace sb
 
-// qkv bf16 `[T, (Hq + 2 Hkv) D]` (row stride ld), q out bf16 `[T, Hq, D]` (row stride q_ld). Pages bf16 (k_scale, v_scale null) or
-// e4m3 `[num_pages, Hkv, page, D]`, rows of D contiguous, with the strides between pages and between heads in elements (scales: between pages). table `[B, P]` (row stride table_ld), lengths `[B]`, starts `[B + 1]` or null (row b is sequence b's). q_gamma, k_gamma
-// null: no norm. cos, sin `[max_pos, D / 2]`, null: no rotation. max_rows: the most rows of one sequence (1 selects the row kernel).
-extern "C" int sb_paged_append(const void* qkv, void* q, const float* q_gamma, const float* k_gamma, const float* cos_t,
-                               const float* sin_t, void* kp, void* vp, float* ks, float* vs, const int* table, const int* lengths,
-                               const int* starts, int T, int B, int P, int Hq, int Hkv, int D, int page, int num_pages, int max_pos,
-                               int max_rows, int zero_tail, float eps, long ld, long q_ld, long table_ld, long k_page, long k_head,
-                               long v_page, long v_head, long ks_ld, long vs_ld, cudaStream_t st) {
+extern "C" int sb_paged_append(const sb::PagedAppendArgs* args) {
   using namespace sb;
-  const int shift = page_shift_of(page);
-  SB_CHECK_ARG((D == 64 || D == 128) && shift >= 0 && Hq > 0 && Hkv > 0 && T > 0 && B > 0 && P > 0 && num_pages > 0 && max_rows > 0);
-  SB_CHECK_ARG(ld % 8 == 0 && q_ld % 8 == 0 && (starts != nullptr || T == B) && (ks == nullptr) == (vs == nullptr));
-  SB_CHECK_ARG((cos_t == nullptr) == (sin_t == nullptr) && (q_gamma == nullptr) == (k_gamma == nullptr) && (cos_t == nullptr || max_pos > 0));
+  SB_CHECK_ARG(args != nullptr);
+  const PagedAppendArgs& c = *args;
+  const int shift = page_shift_of(c.page);
+  SB_CHECK_ARG((c.D == 64 || c.D == 128) && shift >= 0 && c.Hq > 0 && c.Hkv > 0 && c.T > 0 && c.B > 0 && c.P > 0 && c.num_pages > 0);
+  SB_CHECK_ARG(c.ld % 8 == 0 && c.q_ld % 8 == 0 && c.max_rows > 0 && (c.starts != nullptr || c.T == c.B));
+  SB_CHECK_ARG((c.k_scale == nullptr) == (c.v_scale == nullptr) && (c.cos == nullptr) == (c.sin == nullptr));
+  SB_CHECK_ARG((c.q_gamma == nullptr) == (c.k_gamma == nullptr) && (c.cos == nullptr || c.max_pos > 0));
   AppendParams p;
-  p.batch = PagedBatch{table, lengths, starts, table_ld, P, B, T, max_rows, shift, num_pages};
-  p.qkv = static_cast<const __nv_bfloat16*>(qkv); p.ld = ld;
-  p.q = static_cast<__nv_bfloat16*>(q); p.q_ld = q_ld;
-  p.q_gamma = q_gamma; p.k_gamma = k_gamma; p.eps = eps;
-  p.cos_t = cos_t; p.sin_t = sin_t; p.max_pos = cos_t != nullptr ? max_pos : 0x7fffffff;
-  p.kp = kp; p.vp = vp; p.ks = ks; p.vs = vs;
-  p.k_page = k_page; p.k_head = k_head; p.v_page = v_page; p.v_head = v_head;
-  p.ks_ld = ks_ld; p.vs_ld = vs_ld;
-  p.Hq = Hq; p.Hkv = Hkv; p.zero_tail = zero_tail;
+  p.batch = PagedBatch{c.table, c.lengths, c.starts, c.table_ld, c.P, c.B, c.T, c.max_rows, shift, c.num_pages};
+  p.qkv = static_cast<const __nv_bfloat16*>(c.qkv); p.ld = c.ld;
+  p.q = static_cast<__nv_bfloat16*>(c.q); p.q_ld = c.q_ld;
+  p.q_gamma = c.q_gamma; p.k_gamma = c.k_gamma; p.eps = c.eps;
+  p.cos_t = c.cos; p.sin_t = c.sin; p.max_pos = c.cos != nullptr ? c.max_pos : 0x7fffffff;
+  p.kp = c.k; p.vp = c.v; p.ks = c.k_scale; p.vs = c.v_scale;
+  p.k_page = c.k_page; p.k_head = c.k_head; p.v_page = c.v_page; p.v_head = c.v_head;
+  p.ks_ld = c.k_scale_ld; p.vs_ld = c.v_scale_ld;
+  p.Hq = c.Hq; p.Hkv = c.Hkv; p.zero_tail = c.zero_tail;
   p.err = error_word();
   if (!p.err) return SB_ERR_CUDA;
-  return D == 64 ? launch_append<64>(p, starts == nullptr, st) : launch_append<128>(p, starts == nullptr, st);
+  return c.D == 64 ? launch_append<64>(p, c.starts == nullptr, c.stream) : launch_append<128>(p, c.starts == nullptr, c.stream);
 }

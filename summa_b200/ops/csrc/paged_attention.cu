@@ -825,44 +825,40 @@ extern "C" long sb_paged_attention_workspace(int B, int Hkv, int P, int page, in
   return cut ? 2L * ctas * (columns <= 8 ? 8 : 16) * (D + 2) : 0;
 }
 
-// q, o bf16 `[T, Hq, D]` with strides between rows (_ld) and heads in elements; pages and their strides as in sb_paged_append. The rows
-// of the call are in the cache already: row i of sequence b stands at lengths[b] + i and sees the keys j < lengths[b] + rows, with
-// causal those j <= its own position, with window >= 0 those |j - position| <= window. zero_tail: rows behind the last sequence
-// become zeros (otherwise they stay as they are).
-extern "C" int sb_paged_attention(const void* q, const void* kp, const void* vp, const float* ks, const float* vs, void* o, float* work,
-                                  const int* table, const int* lengths, const int* starts, int T, int B, int P, int Hq, int Hkv, int D,
-                                  int page, int num_pages, int max_rows, int causal, int window, int zero_tail, float scale,
-                                  long table_ld, long q_ld, long q_head, long o_ld, long o_head, long k_page, long k_head, long v_page,
-                                  long v_head, long ks_ld, long vs_ld, cudaStream_t st) {
+// The rows of the call are in the cache already: row i of sequence b stands at lengths[b] + i and sees the keys j < lengths[b] + rows,
+// with causal those j <= its own position, with window >= 0 those |j - position| <= window. max_rows * Hq / Hkv is at most 16.
+extern "C" int sb_paged_attention(const sb::PagedAttentionArgs* args) {
   using namespace sb;
-  const int shift = page_shift_of(page);
-  SB_CHECK_ARG((D == 64 || D == 128) && shift >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && T > 0 && B > 0 && P > 0 && num_pages > 0);
-  SB_CHECK_ARG(max_rows > 0 && (starts != nullptr || (T == B && max_rows == 1)) && (ks == nullptr) == (vs == nullptr));
-  SB_CHECK_ARG(max_rows <= 16 && max_rows * (Hq / Hkv) <= 16);
-  // places of the list of work, at the shortest unit, in 32 bits
-  SB_CHECK_ARG((static_cast<double>(P) * page / 64 + 1 + PD_START) * B * Hkv < 2e9);
-  SB_CHECK_ARG(k_page >= 0 && v_page >= 0 && k_head >= 0 && v_head >= 0);
-  const bool fp8 = ks != nullptr;
+  SB_CHECK_ARG(args != nullptr);
+  const PagedAttentionArgs& c = *args;
+  const int shift = page_shift_of(c.page);
+  SB_CHECK_ARG((c.D == 64 || c.D == 128) && shift >= 0 && c.Hq > 0 && c.Hkv > 0 && c.Hq % c.Hkv == 0 && c.T > 0 && c.B > 0 && c.P > 0 && c.num_pages > 0);
+  SB_CHECK_ARG(c.max_rows > 0 && (c.starts != nullptr || (c.T == c.B && c.max_rows == 1)) && (c.k_scale == nullptr) == (c.v_scale == nullptr));
+  SB_CHECK_ARG(c.max_rows <= 16 && c.max_rows * (c.Hq / c.Hkv) <= 16);
+  // places of the list of work in 32 bits, at the shortest unit; a page's stride in 32 bits (unsigned)
+  SB_CHECK_ARG((static_cast<double>(c.P) * c.page / 64 + 1 + PD_START) * c.B * c.Hkv < 2e9);
+  const bool fp8 = c.k_scale != nullptr;
   const long size = fp8 ? 1 : 2;
+  SB_CHECK_ARG(c.k_page >= 0 && c.v_page >= 0 && c.k_head >= 0 && c.v_head >= 0 && c.k_page * size < (1L << 32) && c.v_page * size < (1L << 32));
   PagedAttnParams p;
-  p.batch = PagedBatch{table, lengths, starts, table_ld, P, B, T, max_rows, shift, num_pages};
-  p.q = static_cast<const __nv_bfloat16*>(q); p.q_ld = q_ld; p.q_head = q_head;
-  p.o = static_cast<__nv_bfloat16*>(o); p.o_ld = o_ld; p.o_head = o_head;
-  p.k = static_cast<const uint8_t*>(kp); p.v = static_cast<const uint8_t*>(vp);
-  p.k_page = k_page * size; p.k_head = k_head * size; p.v_page = v_page * size; p.v_head = v_head * size;
-  p.ks = ks; p.vs = vs; p.ks_ld = ks_ld; p.vs_ld = vs_ld;
-  p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
-  p.causal = causal; p.window = window; p.scale_log2 = scale * 1.4426950408889634f;
-  p.zero_tail = zero_tail;
+  p.batch = PagedBatch{c.table, c.lengths, c.starts, c.table_ld, c.P, c.B, c.T, c.max_rows, shift, c.num_pages};
+  p.q = static_cast<const __nv_bfloat16*>(c.q); p.q_ld = c.q_ld; p.q_head = c.q_head;
+  p.o = static_cast<__nv_bfloat16*>(c.o); p.o_ld = c.o_ld; p.o_head = c.o_head;
+  p.k = static_cast<const uint8_t*>(c.k); p.v = static_cast<const uint8_t*>(c.v);
+  p.k_page = c.k_page * size; p.k_head = c.k_head * size; p.v_page = c.v_page * size; p.v_head = c.v_head * size;
+  p.ks = c.k_scale; p.vs = c.v_scale; p.ks_ld = c.k_scale_ld; p.vs_ld = c.v_scale_ld;
+  p.Hq = c.Hq; p.Hkv = c.Hkv; p.G = c.Hq / c.Hkv;
+  p.causal = c.causal; p.window = c.window; p.scale_log2 = c.scale * 1.4426950408889634f;
+  p.zero_tail = c.zero_tail;
   bool cut;
-  p.ctas = paged_decode_ctas(B, Hkv, static_cast<long>(P) * page, D, fp8, &cut);
-  SB_CHECK_ARG(!cut || work != nullptr);
-  p.part = cut ? work : nullptr;
+  p.ctas = paged_decode_ctas(c.B, c.Hkv, static_cast<long>(c.P) * c.page, c.D, fp8, &cut);
+  SB_CHECK_ARG(!cut || c.work != nullptr);
+  p.part = cut ? c.work : nullptr;
   p.err = error_word();
   if (!p.err) return SB_ERR_CUDA;
-  const bool two = max_rows * p.G > 8;
-#define SB_PD(DD, FF) return two ? launch_paged_decode<DD, FF, 2>(p, st) : launch_paged_decode<DD, FF, 1>(p, st)
-  if (D == 64) { if (fp8) SB_PD(64, true); else SB_PD(64, false); }
+  const bool two = c.max_rows * p.G > 8;
+#define SB_PD(DD, FF) return two ? launch_paged_decode<DD, FF, 2>(p, c.stream) : launch_paged_decode<DD, FF, 1>(p, c.stream)
+  if (c.D == 64) { if (fp8) SB_PD(64, true); else SB_PD(64, false); }
   if (fp8) SB_PD(128, true);
   SB_PD(128, false);
 #undef SB_PD

@@ -747,33 +747,32 @@ extern "C" long sb_paged_prefill_workspace(int T, int B, int Hkv, int G, int P, 
   return splits > 1 ? splits * tiles * Hkv * 256L * (D + 2) : 0;
 }
 
-// As sb_paged_attention, for any number of rows per sequence and of query heads per kv head.
-extern "C" int sb_paged_prefill(const void* q, const void* kp, const void* vp, const float* ks, const float* vs, void* o, float* work,
-                                const int* table, const int* lengths, const int* starts, int T, int B, int P, int Hq, int Hkv, int D,
-                                int page, int num_pages, int causal, int window, int zero_tail, float scale, long table_ld, long q_ld,
-                                long q_head, long o_ld, long o_head, long k_page, long k_head, long v_page, long v_head, long ks_ld,
-                                long vs_ld, cudaStream_t st) {
+// As sb_paged_attention, for any number of rows per sequence (max_rows is not read) and of query heads per kv head.
+extern "C" int sb_paged_prefill(const sb::PagedAttentionArgs* args) {
   using namespace sb;
-  const int shift = page_shift_of(page);
-  SB_CHECK_ARG((D == 64 || D == 128) && shift >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && T > 0 && B > 0 && P > 0 && num_pages > 0);
-  SB_CHECK_ARG((starts != nullptr || T == B) && (ks == nullptr) == (vs == nullptr) && scale > 0.f && static_cast<long>(T) * Hq < (1L << 31) - 256);
-  const bool fp8 = ks != nullptr;
+  SB_CHECK_ARG(args != nullptr);
+  const PagedAttentionArgs& c = *args;
+  const int shift = page_shift_of(c.page);
+  SB_CHECK_ARG((c.D == 64 || c.D == 128) && shift >= 0 && c.Hq > 0 && c.Hkv > 0 && c.Hq % c.Hkv == 0 && c.T > 0 && c.B > 0 && c.P > 0 && c.num_pages > 0);
+  SB_CHECK_ARG((c.starts != nullptr || c.T == c.B) && (c.k_scale == nullptr) == (c.v_scale == nullptr) && c.scale > 0.f);
+  SB_CHECK_ARG(static_cast<long>(c.T) * c.Hq < (1L << 31) - 256);
+  const bool fp8 = c.k_scale != nullptr;
   const long size = fp8 ? 1 : 2;
-  SB_CHECK_ARG(k_page >= 0 && v_page >= 0 && k_head >= 0 && v_head >= 0 && k_page * size < (1L << 32) && v_page * size < (1L << 32));
+  SB_CHECK_ARG(c.k_page >= 0 && c.v_page >= 0 && c.k_head >= 0 && c.v_head >= 0 && c.k_page * size < (1L << 32) && c.v_page * size < (1L << 32));
   PagedPrefillParams p;
-  p.batch = PagedBatch{table, lengths, starts, table_ld, P, B, T, T, shift, num_pages};
-  p.q = static_cast<const __nv_bfloat16*>(q); p.q_ld = q_ld; p.q_head = q_head;
-  p.o = static_cast<__nv_bfloat16*>(o); p.o_ld = o_ld; p.o_head = o_head;
-  p.k = static_cast<const uint8_t*>(kp); p.v = static_cast<const uint8_t*>(vp);
-  p.k_page = k_page * size; p.k_head = k_head * size; p.v_page = v_page * size; p.v_head = v_head * size;
-  p.ks = ks; p.vs = vs; p.ks_ld = ks_ld; p.vs_ld = vs_ld;
-  p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
-  p.causal = causal; p.window = window; p.scale_log2 = scale * 1.4426950408889634f;
-  p.zero_tail = zero_tail; p.part = work;
-  p.tiles = paged_prefill_shape(T, B, Hkv, p.G, static_cast<long>(P) * page, &p.splits);
-  SB_CHECK_ARG(p.tiles <= 65535 && (p.splits == 1 || work != nullptr));
+  p.batch = PagedBatch{c.table, c.lengths, c.starts, c.table_ld, c.P, c.B, c.T, c.T, shift, c.num_pages};
+  p.q = static_cast<const __nv_bfloat16*>(c.q); p.q_ld = c.q_ld; p.q_head = c.q_head;
+  p.o = static_cast<__nv_bfloat16*>(c.o); p.o_ld = c.o_ld; p.o_head = c.o_head;
+  p.k = static_cast<const uint8_t*>(c.k); p.v = static_cast<const uint8_t*>(c.v);
+  p.k_page = c.k_page * size; p.k_head = c.k_head * size; p.v_page = c.v_page * size; p.v_head = c.v_head * size;
+  p.ks = c.k_scale; p.vs = c.v_scale; p.ks_ld = c.k_scale_ld; p.vs_ld = c.v_scale_ld;
+  p.Hq = c.Hq; p.Hkv = c.Hkv; p.G = c.Hq / c.Hkv;
+  p.causal = c.causal; p.window = c.window; p.scale_log2 = c.scale * 1.4426950408889634f;
+  p.zero_tail = c.zero_tail; p.part = c.work;
+  p.tiles = paged_prefill_shape(c.T, c.B, c.Hkv, p.G, static_cast<long>(c.P) * c.page, &p.splits);
+  SB_CHECK_ARG(p.tiles <= 65535 && (p.splits == 1 || c.work != nullptr));
   p.err = error_word();
   if (!p.err) return SB_ERR_CUDA;
-  if (D == 64) return fp8 ? launch_paged_prefill<64, true>(p, st) : launch_paged_prefill<64, false>(p, st);
-  return fp8 ? launch_paged_prefill<128, true>(p, st) : launch_paged_prefill<128, false>(p, st);
+  if (c.D == 64) return fp8 ? launch_paged_prefill<64, true>(p, c.stream) : launch_paged_prefill<64, false>(p, c.stream);
+  return fp8 ? launch_paged_prefill<128, true>(p, c.stream) : launch_paged_prefill<128, false>(p, c.stream);
 }

@@ -12,6 +12,7 @@ import ctypes
 import functools
 import os
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -581,44 +582,51 @@ def decode_attention(q, k, v, causal, window, q_offset, scale=None):
     return o
 
 
-N.register("sb_paged_append", [N.P] * 13 + [N.I] * 11 + [N.F] + [N.L] * 9 + [N.P])
-N.register("sb_paged_attention", [N.P] * 10 + [N.I] * 12 + [N.F] + [N.L] * 11 + [N.P])
+N.register("sb_paged_append", [N.P])
+N.register("sb_paged_attention", [N.P])
+N.register("sb_paged_prefill", [N.P])
 N.register("sb_paged_attention_workspace", [N.I] * 7, restype=ctypes.c_long)
-
-
-def _cache_strides(kv):
-    """(k page, k head, v page, v head, k_scale page, v_scale page) in elements."""
-    k, v, ks, vs = kv
-    a, b = k.stride(), v.stride()
-    return a[0], a[1], b[0], b[1], 0 if ks is None else ks.stride(0), 0 if vs is None else vs.stride(0)
+N.register("sb_paged_prefill_workspace", [N.I] * 7, restype=ctypes.c_long)
+# The arguments of a call as the C side's structs (PagedAppendArgs, PagedAttentionArgs): packed at once, they take a third of the time
+# that as many arguments of a foreign call do.
+_PAGED_APPEND = struct.Struct("=14Q9q11if")
+_PAGED_ATTENTION = struct.Struct("=11Q11q12ifi")
+PAGED_COLUMNS = 16      # rows of a sequence times query heads of a kv head that the streaming kernel takes; beyond, the tiled one
 
 
 def _heads_ok(t: torch.Tensor) -> bool:
     """Rows of heads `[T, H, D]` whose heads begin on 16 bytes."""
-    s = t.stride()
-    return s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0
+    a, b, c = t.stride()
+    return c == 1 and (a | b) % 8 == 0 and t.data_ptr() % 16 == 0
 
 
-def paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv, rows, out=None):
-    """See `ops.paged_append`."""
-    if qkv.device.index != torch.cuda.current_device():
-        with torch.cuda.device(qkv.device):
-            return paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv, rows, out)
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv, rows, layout, out=None):
+    """See `ops.paged_append`; `layout` from its checks."""
+    device = qkv.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv, rows, layout, out)
     T = qkv.shape[0]
-    if out is not None and not (_heads_ok(out) and out.stride(1) == D):
-        q = out.contiguous()
-        q = q.clone() if q.data_ptr() % 16 else q
+    if out is None:
+        q, q_ld = torch.empty(T, Hq, D, device=device, dtype=BF16), Hq * D
+    elif _heads_ok(out) and out.stride(1) == D:
+        q, q_ld = out, out.stride(0)
     else:
-        q = torch.empty(T, Hq, D, device=qkv.device, dtype=BF16) if out is None else out
+        q = out.contiguous()
+        q, q_ld = q.clone() if q.data_ptr() % 16 else q, Hq * D
     if T > 0:
         x, ld = _rows(qkv)
         qg, kg = (None, None) if q_gamma is None else (_gains(q_gamma), _gains(k_gamma))
         k, v, ks, vs = kv
-        table, lengths, starts, _ = rows
-        N.call("sb_paged_append", x.data_ptr(), q.data_ptr(), N.ptr(qg), N.ptr(kg), N.ptr(cos), N.ptr(sin), k.data_ptr(), v.data_ptr(),
-               N.ptr(ks), N.ptr(vs), table.data_ptr(), lengths.data_ptr(), N.ptr(starts), T, table.shape[0], table.shape[1], Hq, Hkv, D,
-               k.shape[2], k.shape[0], cos.shape[0] if cos is not None else 0, rows.most(T), 1 if out is None else 0, eps, ld, q.stride(0),
-               table.stride(0), *_cache_strides(kv), N.stream())
+        B, P, page, pages, table_ld, k_page, k_head, v_page, v_head, ks_ld, vs_ld = layout
+        N.call("sb_paged_append", _PAGED_APPEND.pack(
+            N.stream(), x.data_ptr(), q.data_ptr(), _at(qg), _at(kg), _at(cos), _at(sin), k.data_ptr(), v.data_ptr(), _at(ks), _at(vs),
+            rows.table.data_ptr(), rows.lengths.data_ptr(), _at(rows.starts), ld, q_ld, table_ld, k_page, k_head, v_page, v_head, ks_ld, vs_ld,
+            T, B, P, Hq, Hkv, D, page, pages, 0 if cos is None else cos.shape[0], rows.most(T), 1 if out is None else 0, eps))
     if out is not None and q is not out:
         out.copy_(q)
     return q if out is None else out
@@ -630,45 +638,42 @@ def _gains(g: torch.Tensor) -> torch.Tensor:
     return g.clone() if g.data_ptr() % 16 else g
 
 
-N.register("sb_paged_prefill", [N.P] * 10 + [N.I] * 11 + [N.F] + [N.L] * 11 + [N.P])
-N.register("sb_paged_prefill_workspace", [N.I] * 7, restype=ctypes.c_long)
-PAGED_COLUMNS = 16      # rows of a sequence times query heads of a kv head that the streaming kernel takes; beyond, the tiled one
-
-
 @functools.lru_cache(maxsize=256)
 def _paged_workspace(device, name, *sizes):
     return N.call_value(name, *sizes)
 
 
-def paged_attention(q, kv, rows, causal=True, window=None, scale=None, out=None):
-    """See `ops.paged_attention`."""
-    device = q.device.index
-    if device != torch.cuda.current_device():
+def paged_attention(q, kv, rows, layout, causal=True, window=None, scale=None, out=None):
+    """See `ops.paged_attention`; `layout` from its checks."""
+    device = q.device
+    if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return paged_attention(q, kv, rows, causal, window, scale, out)
+            return paged_attention(q, kv, rows, layout, causal, window, scale, out)
     T, Hq, D = q.shape
     q = q if _heads_ok(q) else q.clone(memory_format=torch.contiguous_format)
-    if out is not None and not _heads_ok(out):
-        o = out.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        o = torch.empty(T, Hq, D, device=device, dtype=BF16)
     else:
-        o = torch.empty(T, Hq, D, device=q.device, dtype=BF16) if out is None else out
+        o = out if _heads_ok(out) else out.clone(memory_format=torch.contiguous_format)
     if T > 0:
         k, v, ks, vs = kv
-        table, lengths, starts, _ = rows
-        pages, Hkv, page, _ = k.shape
-        B, P = table.shape
-        most, G = rows.most(T), Hq // Hkv
+        B, P, page, pages, table_ld, k_page, k_head, v_page, v_head, ks_ld, vs_ld = layout
+        Hkv, most = k.shape[1], rows.most(T)
+        G = Hq // Hkv
         if most * G <= PAGED_COLUMNS:
-            name, most = "sb_paged_attention", (most,)
-            need = _paged_workspace(device, "sb_paged_attention_workspace", B, Hkv, P, page, D, 0 if ks is None else 1, most[0] * G)
+            name = "sb_paged_attention"
+            need = _paged_workspace(device.index, "sb_paged_attention_workspace", B, Hkv, P, page, D, 0 if ks is None else 1, most * G)
         else:
-            name, most = "sb_paged_prefill", ()
-            need = _paged_workspace(device, "sb_paged_prefill_workspace", T, B, Hkv, G, P, page, D)
-        ws = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
-        N.call(name, q.data_ptr(), k.data_ptr(), v.data_ptr(), N.ptr(ks), N.ptr(vs), o.data_ptr(), N.ptr(ws),
-               table.data_ptr(), lengths.data_ptr(), N.ptr(starts), T, B, P, Hq, Hkv, D, page, pages, *most, 1 if causal else 0,
-               -1 if window is None else min(int(window), 0x7fffffff), 1 if out is None else 0, 1.0 / math.sqrt(D) if scale is None else scale,
-               table.stride(0), q.stride(0), q.stride(1), o.stride(0), o.stride(1), *_cache_strides(kv), N.stream())
+            name = "sb_paged_prefill"
+            need = _paged_workspace(device.index, "sb_paged_prefill_workspace", T, B, Hkv, G, P, page, D)
+        ws = torch.empty(need, device=device, dtype=torch.float32) if need else None
+        q_ld, q_head, _ = q.stride()
+        o_ld, o_head, _ = o.stride()
+        N.call(name, _PAGED_ATTENTION.pack(
+            N.stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(ks), _at(vs), o.data_ptr(), _at(ws), rows.table.data_ptr(),
+            rows.lengths.data_ptr(), _at(rows.starts), q_ld, q_head, o_ld, o_head, table_ld, k_page, k_head, v_page, v_head, ks_ld, vs_ld,
+            T, B, P, Hq, Hkv, D, page, pages, most, 1 if causal else 0, -1 if window is None else min(int(window), 0x7fffffff),
+            1 if out is None else 0, 1.0 / math.sqrt(D) if scale is None else scale, 0))
     if out is not None and o is not out:
         out.copy_(o)
     return o if out is None else out

@@ -41,9 +41,25 @@ class PagedRows(NamedTuple):
         return 1 if self.starts is None else total if self.max_rows is None else min(int(self.max_rows), total)
 
 
-# (the checks run in front of every launch of a decoding step, so a message is only put together where one fails)
+# (The checks run in front of every launch of a decoding step: a message is only put together where one fails, and what they look up
+# is handed on.)
 
-def check(x: torch.Tensor, Hkv: int, D: int, kv: PagedKV, rows: PagedRows) -> None:
+class Layout(NamedTuple):
+    """What a launch needs to know of the tensors, in its order: sizes, then strides in elements."""
+    sequences: int
+    table_pages: int
+    page: int
+    num_pages: int
+    table_ld: int
+    k_page: int
+    k_head: int
+    v_page: int
+    v_head: int
+    k_scale_ld: int
+    v_scale_ld: int
+
+
+def check(x: torch.Tensor, Hkv: int, D: int, kv: PagedKV, rows: PagedRows) -> Layout:
     """The checks that both calls share; `x` is what has a row per token."""
     k, v, k_scale, v_scale = kv
     table, lengths, starts, max_rows = rows
@@ -55,15 +71,32 @@ def check(x: torch.Tensor, Hkv: int, D: int, kv: PagedKV, rows: PagedRows) -> No
         raise ValueError(f"pages of {heads} heads of {d}, and rows of {Hkv} heads of {D}")
     if page not in PAGE_SIZES:
         raise ValueError(f"page size {page}: one of {PAGE_SIZES}")
+    k_page, k_head, k_row, k_one = k.stride()
+    v_page, v_head, v_row, v_one = v.stride()
+    if k_one != 1 or v_one != 1 or k_row != D or v_row != D or k.device != device or v.device != device:
+        raise ValueError("the rows of a page and head have to lie together, on the device of the rows of the call")
+    ks_ld = vs_ld = 0
     if dtype == E4M3:
-        for s in (k_scale, v_scale):
-            if s is None or s.dtype != torch.float32 or s.shape != (pages, heads) or s.stride(1) != 1 or s.device != device:
-                raise ValueError(f"e4m3 pages need fp32 scales [{pages}, {heads}] with adjacent heads, on the device of the rows")
-    elif dtype != x.dtype or k_scale is not None or v_scale is not None:
-        raise ValueError(f"pages of {dtype} for rows of {x.dtype}: of the same type without scales, or e4m3 with them")
-    if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1 or table.device != device:
-        raise ValueError("table: int32 [B, P] with adjacent pages, on the device of the rows")
-    B = table.shape[0]
+        unit = 16
+        if (k_scale is None or v_scale is None or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32
+                or k_scale.shape != (pages, heads) or v_scale.shape != (pages, heads) or k_scale.device != device or v_scale.device != device):
+            raise ValueError(f"e4m3 pages need fp32 scales [{pages}, {heads}] on the device of the rows")
+        ks_ld, one = k_scale.stride()
+        vs_ld, two = v_scale.stride()
+        if one != 1 or two != 1:
+            raise ValueError("the scales of a page's heads have to lie together")
+    else:
+        unit = 8
+        if dtype != x.dtype or k_scale is not None or v_scale is not None:
+            raise ValueError(f"pages of {dtype} for rows of {x.dtype}: of the same type without scales, or e4m3 with them")
+    if x.is_cuda and (k.data_ptr() % 16 or v.data_ptr() % 16 or (k_page | k_head | v_page | v_head) % unit):
+        raise ValueError("pages and heads have to begin on 16 bytes")
+    if table.dim() != 2 or table.dtype != torch.int32 or table.device != device:
+        raise ValueError("table: int32 [B, P] on the device of the rows")
+    B, P = table.shape
+    table_ld, one = table.stride()
+    if one != 1:
+        raise ValueError("the pages of a sequence in the table have to lie together")
     if lengths.dtype != torch.int32 or lengths.shape != (B,) or not lengths.is_contiguous() or lengths.device != device:
         raise ValueError(f"lengths: int32 [{B}] on the device of the rows")
     if starts is None:
@@ -73,16 +106,10 @@ def check(x: torch.Tensor, Hkv: int, D: int, kv: PagedKV, rows: PagedRows) -> No
         raise ValueError(f"starts: int32 [{B + 1}] on the device of the rows")
     if max_rows is not None and max_rows < 1:
         raise ValueError(f"max_rows {max_rows}")
-    size = 1 if dtype == E4M3 else 2
-    for t in (k, v):
-        s = t.stride()
-        if s[3] != 1 or s[2] != D or t.device != device:
-            raise ValueError("the rows of a page and head have to lie together, on the device of the rows of the call")
-        if t.is_cuda and (t.data_ptr() % 16 or s[0] * size % 16 or s[1] * size % 16):
-            raise ValueError("pages and heads have to begin on 16 bytes")
+    return Layout(B, P, page, pages, table_ld, k_page, k_head, v_page, v_head, ks_ld, vs_ld)
 
 
-def check_append(qkv, q_gamma, k_gamma, cos, sin, Hq, Hkv, D, kv, rows, out) -> None:
+def check_append(qkv, q_gamma, k_gamma, cos, sin, Hq, Hkv, D, kv, rows, out) -> Layout:
     device = qkv.device
     if qkv.dim() != 2 or Hq < 1 or Hkv < 1 or qkv.shape[1] != (Hq + 2 * Hkv) * D:
         raise ValueError(f"qkv: [T, ({Hq} + 2 * {Hkv}) * {D}], got {list(qkv.shape)}")
@@ -91,21 +118,24 @@ def check_append(qkv, q_gamma, k_gamma, cos, sin, Hq, Hkv, D, kv, rows, out) -> 
     if q_gamma is not None and not (q_gamma.shape == k_gamma.shape == (D,) and q_gamma.device == k_gamma.device == device):
         raise ValueError(f"gains of a head: [{D}], on the device of the rows")
     if cos is not None:
-        for t in (cos, sin):
-            if t.dim() != 2 or t.shape[1] != D // 2 or t.shape != cos.shape or t.dtype != torch.float32 or not t.is_contiguous() \
-                    or t.device != device or (t.is_cuda and t.data_ptr() % 16):
-                raise ValueError(f"cos, sin: fp32 [positions, {D // 2}], contiguous and on the device of the rows")
+        shape = cos.shape
+        if (len(shape) != 2 or shape[1] != D // 2 or sin.shape != shape or cos.dtype != torch.float32 or sin.dtype != torch.float32
+                or not cos.is_contiguous() or not sin.is_contiguous() or cos.device != device or sin.device != device):
+            raise ValueError(f"cos, sin: fp32 [positions, {D // 2}], contiguous and on the device of the rows")
+        if cos.is_cuda and (cos.data_ptr() % 16 or sin.data_ptr() % 16):
+            raise ValueError("cos and sin have to begin on 16 bytes")
         if cos.shape[0] < 1:
             raise ValueError("cos, sin: no position")
     if out is not None and (out.shape != (qkv.shape[0], Hq, D) or out.dtype != qkv.dtype or out.device != device):
         raise ValueError(f"out: [{qkv.shape[0]}, {Hq}, {D}] of the type and device of the rows")
-    check(qkv, Hkv, D, kv, rows)
+    return check(qkv, Hkv, D, kv, rows)
 
 
-def check_attention(q, kv, rows, window, scale, out) -> None:
+def check_attention(q, kv, rows, window, scale, out) -> Layout:
     if q.dim() != 3 or kv.k.dim() != 4:
         raise ValueError("q: [T, Hq, D]; pages: [num_pages, Hkv, page, D]")
-    Hq, Hkv = q.shape[1], kv.k.shape[1]
+    _, Hq, D = q.shape
+    Hkv = kv.k.shape[1]
     if Hq < 1 or Hkv < 1 or Hq % Hkv:
         raise ValueError(f"{Hq} query heads over {Hkv} kv heads")
     if window is not None and window < 0:
@@ -114,7 +144,7 @@ def check_attention(q, kv, rows, window, scale, out) -> None:
         raise ValueError(f"scale {scale}: it has to be positive")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device):
         raise ValueError(f"out: {list(q.shape)} of the type and device of the rows")
-    check(q, Hkv, q.shape[2], kv, rows)
+    return check(q, Hkv, D, kv, rows)
 
 
 # ------------------------------------------------------------------ PyTorch form (CPU tensors)
