@@ -411,49 +411,58 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem_base + a * 64 + lane_sel, t_o = tmem_base + C::COL_O + a * D + lane_sel;
 
-    {
-      // The query rows into their tiles: D / 8 threads a row. In 8 bits as f16, scaled by a power of two, whose inverse goes to the row's thread.
-      float* backs = reinterpret_cast<float*>(smem + C::OFF_BACK);
-      constexpr int TPR = D / 8, RPS = 256 / TPR, STEPS = 256 / RPS;
-      uint4 w[STEPS];
-      const int c = threadIdx.x % TPR;
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const unsigned x = x0 + i * RPS + threadIdx.x / TPR;
-        w[i] = make_uint4(0, 0, 0, 0);
-        if (x < pairs) {
-          const unsigned row = x / G, head = kh * G + x % G;
-          w[i] = *reinterpret_cast<const uint4*>(p.q + (tl.row0 + row) * p.q_ld + head * p.q_head + c * 8);
-        }
+    // The query rows into the group's tile, a warp its own 32: D / 8 threads a row. In 8 bits a thread then turns its row to f16, scaled by a
+    // power of two, whose inverse it keeps. (What runs once per tile is kept in short loops: unrolled over registers this was 11,000 cycles of
+    // a tile, most of them instruction fetches.)
+    const uint32_t back_at = smem_u32(smem + C::OFF_BACK) + threadIdx.x * 4;
+    const int wr = warp & 3;
+    // (the tile's first row stands in for a pair that is none)
+    auto pair_offset = [&](long ld, long head_ld) { return (tl.row0 + (live ? x : x0) / G) * ld + (kh * G + (live ? x : x0) % G) * head_ld; };
+    if (a < tiles_here) {
+      constexpr int TPR = D / 8, RPS = 32 / TPR;
+      const int c = lane % TPR;
+      const long mine = pair_offset(p.q_ld, p.q_head);
+      const unsigned there = __ballot_sync(0xffffffffu, live);
+      uint8_t* tile = smem + a * C::TILE + wr * 32 * 128;
+#pragma unroll 4
+      for (int r0 = 0; r0 < 32; r0 += RPS) {
+        const int r = r0 + lane / TPR;
+        const long at = __shfl_sync(0xffffffffu, mine, r);
+        cp_async16_zfill(smem_u32(tile + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)), p.q + at + c * 8, there >> r & 1 ? 16 : 0);
       }
+      cp_async_commit();
+      cp_async_wait_group<0>();
+      if (FP8) {
+        __syncwarp();
+        __nv_bfloat162 most2 = __float2bfloat162_rn(0.f);
+        auto chunk = [&](int k) { return reinterpret_cast<uint4*>(tile + (k >> 3) * 16384 + lane * 128 + (((k & 7) ^ (lane & 7)) << 4)); };
+#pragma unroll 4
+        for (int k = 0; k < TPR; ++k) {
+          const uint4 w = *chunk(k);
+          const uint32_t u[4] = {w.x & 0x7fff7fffu, w.y & 0x7fff7fffu, w.z & 0x7fff7fffu, w.w & 0x7fff7fffu};
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int r = i * RPS + threadIdx.x / TPR;
-        if (FP8) {
-          uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-          float most = 0.f;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) most = fmaxf(most, fmaxf(fabsf(bf16_lo(u[k])), fabsf(bf16_hi(u[k]))));
-#pragma unroll
-          for (int k = TPR / 2; k > 0; k >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, k, TPR));
-          int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100);
-          if (most == 0.f || !(most < INFINITY)) e = 14;
-          const float mul = exp_scale(14 - e);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const __half2 h = __floats2half2_rn(bf16_lo(u[k]) * mul, bf16_hi(u[k]) * mul);
-            u[k] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-          w[i] = make_uint4(u[0], u[1], u[2], u[3]);
-          if (c == 0) backs[r] = exp_scale(e - 14);
+          for (int i = 0; i < 4; ++i) most2 = __hmax2(most2, *reinterpret_cast<const __nv_bfloat162*>(&u[i]));
         }
-        *reinterpret_cast<uint4*>(smem + (r >> 7) * C::TILE + (c >> 3) * 16384 + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = w[i];
+        const float most = fmaxf(__low2float(most2), __high2float(most2));
+        int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100);
+        if (most == 0.f || !(most < INFINITY)) e = 14;
+        const float mul = exp_scale(14 - e);
+        asm volatile("st.shared.f32 [%0], %1;" :: "r"(back_at), "f"(p.scale_log2 * exp_scale(e - 14)) : "memory");
+#pragma unroll 2
+        for (int k = 0; k < TPR; ++k) {
+          const uint4 w = *chunk(k);
+          uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(bf16_lo(u[i]) * mul, bf16_hi(u[i]) * mul);
+            u[i] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          *chunk(k) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
       }
       fence_proxy_async_smem();
-      warp_arrive(q_full);
-      if (FP8) asm volatile("bar.sync 1, 256;" ::: "memory");     // (no wait in front of it that could give up)
     }
-    const float back = FP8 ? p.scale_log2 * reinterpret_cast<const float*>(smem + C::OFF_BACK)[a * 128 + t] : p.scale_log2;
+    warp_arrive(q_full);
 
     // keys that this pair sees: [klo, khi)
     const long pos = static_cast<long>(tl.len) + row;
@@ -477,6 +486,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       // factor and exponent of the four groups of 16 keys (bf16 pages: the softmax scale and 0)
       const uint32_t sc = smem_u32(scales) + (i % C::RING) * 64;
       float fs[4], e[4], inv[4];
+      float back = p.scale_log2;
+      if (FP8) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(back) : "r"(back_at) : "memory");
       bool masked = kv0 < klo || kv0 + PP_KEYS > khi;
 #pragma unroll
       for (int gp = 0; gp < 4; ++gp) {
@@ -585,9 +596,9 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     // The rows leave through shared memory (the group's query tile: its products are done), so that a row's bytes are stored side by
     // side; a warp has 32 rows of 2 D bytes there: a bf16 row, or half a row in 32 bits.
     constexpr int CH = D / 8;                    // 16-byte chunks of those
-    uint8_t* mine = smem + a * C::TILE + (warp & 3) * (32 * D * 2);
+    uint8_t* stage = smem + a * C::TILE + wr * (32 * D * 2);
     const unsigned xw = x0 + a * 128 + (warp & 3) * 32;
-    auto staged = [&](int r, int c) { return reinterpret_cast<uint4*>(mine + r * (D * 2) + ((c ^ (r & (CH - 1))) << 4)); };
+    auto staged = [&](int r, int c) { return reinterpret_cast<uint4*>(stage + r * (D * 2) + ((c ^ (r & (CH - 1))) << 4)); };
     if (p.splits > 1) {
       const size_t at = ((static_cast<size_t>(blockIdx.z) * p.tiles + blockIdx.y) * p.Hkv + kh) * 256 + a * 128;
       float* ml = p.part + static_cast<size_t>(p.splits) * p.tiles * p.Hkv * 256 * D + (at + t) * 2;
@@ -595,7 +606,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       if (__all_sync(0xffffffffu, have)) {       // (what has no keys is not read again)
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
-#pragma unroll
+#pragma unroll 1
           for (int cc = 0; cc < D / 32; ++cc) {
             uint32_t o16[16];
             tmem_ld_32x32b_x16(t_o + h * (D / 2) + cc * 16, o16);
@@ -616,7 +627,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     } else {
       // (a sum of nothing: no key, zeros; a NaN stays one)
       const float inv_l = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
+      const long mine = pair_offset(p.o_ld, p.o_head);
+#pragma unroll 1
       for (int cc = 0; cc < D / 16; ++cc) {
         uint32_t o16[16];
         if (__all_sync(0xffffffffu, have)) {
@@ -640,9 +652,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
 #pragma unroll 4
       for (int i = 0; i < CH; ++i) {
         const int r = i * (32 / CH) + lane / CH, c = lane % CH;
-        const unsigned y = xw + r;
-        if (y < pairs)
-          *reinterpret_cast<uint4*>(p.o + (tl.row0 + y / G) * p.o_ld + (kh * G + y % G) * p.o_head + c * 8) = *staged(r, c);
+        const long at = __shfl_sync(0xffffffffu, mine, r);
+        if (xw + r < pairs) *reinterpret_cast<uint4*>(p.o + at + c * 8) = *staged(r, c);
       }
     }
   }
