@@ -81,16 +81,22 @@ __device__ __forceinline__ void norm_rotate(float* v, const AppendParams& p, con
   }
 }
 
-// The largest finite magnitude of 8 values; anything infinite becomes NaN on the way, which is how a page holds it.
+// The largest finite magnitude of 8 values; anything infinite becomes NaN on the way, which is how a page holds it. (Magnitudes of floats
+// are ordered as their bits are.)
 __device__ __forceinline__ float finite_max(float* v) {
-  float m = 0.f;
+  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = fabsf(v[i]);
-    if (!(a < INFINITY)) v[i] = __uint_as_float(0x7fffffffu);
-    else m = fmaxf(m, a);
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  if (m >= 0x7f800000u) {
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+      if (a >= 0x7f800000u) v[i] = __uint_as_float(0x7fffffffu);
+      else m = max(m, a);
+    }
   }
-  return m;
+  return __uint_as_float(m);
 }
 
 __device__ __forceinline__ uint2 encode8(const float* v, float inv) {
@@ -216,32 +222,44 @@ __global__ void __launch_bounds__(256, NP > 4 ? 2 : 4) paged_append_segments_ker
   const int shift = p.batch.page_shift;
   int seg = (blockIdx.x - q_blocks) / (2 * p.Hkv), b = -1;
   const int h = (blockIdx.x - q_blocks) % (2 * p.Hkv);
-  // every warp finds the segment by itself: segments of 32 sequences at a time, summed over the lanes
-  PagedSeq s;
-  for (int b0 = 0; b0 < p.batch.B && b < 0; b0 += 32) {
-    int n = 0;
-    s = PagedSeq{0, 0, -1};
-    if (b0 + lane < p.batch.B) {
-      s = paged_seq(p.batch, b0 + lane);
-      if (s.rows > 0 && s.len >= 0) n = static_cast<int>(((static_cast<long>(s.len) + s.rows - 1) >> shift) - (s.len >> shift)) + 1;
-    }
-    int sum = n;
+  // warp 0 finds the segment: segments of 32 sequences at a time, summed over the lanes
+  __shared__ int found[5];
+  if (warp == 0) {
+    PagedSeq s;
+    for (int b0 = 0; b0 < p.batch.B && b < 0; b0 += 32) {
+      int n = 0;
+      s = PagedSeq{0, 0, -1};
+      if (b0 + lane < p.batch.B) {
+        s = paged_seq(p.batch, b0 + lane);
+        if (s.rows > 0 && s.len >= 0) n = static_cast<int>(((static_cast<long>(s.len) + s.rows - 1) >> shift) - (s.len >> shift)) + 1;
+      }
+      int sum = n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+      }
+      const int all = __shfl_sync(0xffffffffu, sum, 31);
+      if (seg < all) {
+        const int l = __popc(__ballot_sync(0xffffffffu, sum <= seg));      // the first lane whose sum passes it
+        b = b0 + l;
+        if (lane == l) {
+          found[1] = seg - (sum - n);
+          found[2] = s.row0;
+          found[3] = s.rows;
+          found[4] = s.len;
+        }
+      } else {
+        seg -= all;
+      }
     }
-    const int all = __shfl_sync(0xffffffffu, sum, 31);
-    if (seg < all) {
-      const int l = __popc(__ballot_sync(0xffffffffu, sum <= seg));      // the first lane whose sum passes it
-      b = b0 + l;
-      seg -= __shfl_sync(0xffffffffu, sum - n, l);
-      s = PagedSeq{__shfl_sync(0xffffffffu, s.row0, l), __shfl_sync(0xffffffffu, s.rows, l), __shfl_sync(0xffffffffu, s.len, l)};
-    } else {
-      seg -= all;
-    }
+    if (lane == 0) found[0] = b;
   }
+  __syncthreads();
+  b = found[0];
   if (b < 0) return;
+  seg = found[1];
+  const PagedSeq s = PagedSeq{found[2], found[3], found[4]};
   const long first = s.len, page_no = (first >> shift) + seg, pos0 = max(first, page_no << shift);
   const int slot0 = static_cast<int>(pos0 - (page_no << shift));
   const int n = static_cast<int>(min(first + s.rows, (page_no + 1) << shift) - pos0);

@@ -50,7 +50,7 @@ struct PagedPrefillParams {
   unsigned int* err;
 };
 
-constexpr int PP_THREADS = 512, PP_KEYS = 64;
+constexpr int PP_THREADS = 512, PP_KEYS = 64, PP_JOIN = 16;
 template <int D, bool FP8>
 struct PagedPrefill {
   static constexpr int TILE = 128 * D * 2, KTILE = PP_KEYS * D * 2;
@@ -727,7 +727,7 @@ static int launch_paged_prefill(PagedPrefillParams& p, cudaStream_t st) {
   cfg.numAttrs = 1;
   SB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_prefill_kernel<D, FP8>, static_cast<const PagedPrefillParams>(p)));
   if (p.splits > 1) {
-    cfg.gridDim = dim3(p.Hkv, p.tiles, 4);
+    cfg.gridDim = dim3(p.Hkv, p.tiles, PP_JOIN);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     SB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_prefill_join_kernel<D>, static_cast<const PagedPrefillParams>(p)));

@@ -6,7 +6,7 @@ its fraction of the measured peaks (`MEASURED_PEAKS.json` beside the package's p
 directory when present, otherwise the stated fallback). `--once` runs two untimed
 launches and exits: the small, bounded workload a profiler capture wants.
 
-Ops: gemm, attention_fwd, attention_bwd, attention_decode, scan, rmsnorm, swiglu, cross_entropy, int4_gemv.
+Ops: gemm, attention_fwd, attention_bwd, attention_decode, paged_append, paged_attention, scan, rmsnorm, swiglu, cross_entropy, int4_gemv.
 """
 from __future__ import annotations
 
@@ -269,7 +269,49 @@ def bench_attention_decode(a):
     _report("attention_decode", timeit(fn, a.iters), nbytes=4.0 * B * Sk * KV * D, B=B, Sk=Sk, H=H, KV=KV)
 
 
+def _paged(a):
+    """B sequences of S tokens in shuffled pages of 64 (head_dim `--D`, elements `--kind`), and M rows of each."""
+    from . import PagedKV, PagedRows
+    H, KV, D, page = a.H, a.KV or a.H, a.D, 64
+    per = -(-(a.S + a.M) // page)
+    pool = torch.randn(2, a.B * per, KV, page, D, device="cuda")
+    if a.kind == "e4m3":
+        scale = torch.ones(2, a.B * per, KV, device="cuda")
+        kv = PagedKV(pool[0].to(torch.float8_e4m3fn), pool[1].to(torch.float8_e4m3fn), scale[0], scale[1])
+    else:
+        kv = PagedKV(pool[0].bfloat16(), pool[1].bfloat16())
+    starts = None if a.M == 1 else torch.arange(a.B + 1, device="cuda", dtype=torch.int32) * a.M
+    rows = PagedRows(torch.randperm(a.B * per, device="cuda").int().view(a.B, per), torch.full((a.B,), a.S, device="cuda", dtype=torch.int32), starts, a.M)
+    return kv, rows, H, KV, D
+
+
+def bench_paged_append(a):
+    from . import paged_append
+    kv, rows, H, KV, D = _paged(a)
+    T, size = a.B * a.M, kv.k.element_size()
+    qkv = torch.randn(T, (H + 2 * KV) * D, device="cuda").bfloat16()
+    angle = torch.rand(a.S + a.M, D // 2, device="cuda")
+    cos, sin = angle.cos(), angle.sin()
+    fn = lambda: paged_append(qkv, None, None, 1e-5, cos, sin, H, KV, D, kv, rows)
+    if a.once:
+        fn(); fn(); return
+    _report("paged_append", timeit(fn, a.iters), nbytes=T * D * (4.0 * H + (4.0 + 2 * size) * KV + 4), B=a.B, S=a.S, M=a.M, H=H, KV=KV, D=D, kind=a.kind)
+
+
+def bench_paged_attention(a):
+    from . import paged_attention
+    kv, rows, H, KV, D = _paged(a)
+    q = torch.randn(a.B * a.M, H, D, device="cuda").bfloat16()
+    fn = lambda: paged_attention(q, kv, rows)
+    if a.once:
+        fn(); fn(); return
+    keys = a.M * a.S + a.M * (a.M + 1) / 2                     # of all rows of a sequence
+    _report("paged_attention", timeit(fn, a.iters), flops=4.0 * a.B * H * D * keys,
+            nbytes=2.0 * a.B * (a.S + a.M) * KV * D * kv.k.element_size() + 4.0 * a.B * a.M * H * D, B=a.B, S=a.S, M=a.M, H=H, KV=KV, D=D, kind=a.kind)
+
+
 OPS = {"gemm": bench_gemm, "attention_decode": bench_attention_decode, "attention_fwd": bench_attention_fwd, "attention_bwd": bench_attention_bwd,
+       "paged_append": bench_paged_append, "paged_attention": bench_paged_attention,
        "scan": bench_scan, "rmsnorm": bench_rmsnorm, "swiglu": bench_swiglu,
        "cross_entropy": bench_cross_entropy, "int4_gemv": bench_int4_gemv, "int4_prefill": bench_int4_prefill}
 
@@ -282,6 +324,7 @@ def main(argv=None):
         ap.add_argument(f"--{name}", type=int, default=default)
     ap.add_argument("--tile", type=int, default=-1, help="gemm: 128 / 256 single-CTA tiles, 512 paired CTAs, 0 auto")
     ap.add_argument("--layout", default="fwd", choices=["fwd", "dgrad", "wgrad"], help="gemm operand layouts")
+    ap.add_argument("--kind", default="e4m3", choices=["e4m3", "bf16"], help="paged_*: the pages' elements (M: rows of each of B sequences behind S tokens)")
     ap.add_argument("--sweep", action="store_true", help="gemm: 8192^3 and the llama-350m training shapes")
     ap.add_argument("--once", action="store_true", help="two untimed launches, for a profiler capture")
     ap.add_argument("--compare", action="store_true", help="also time the library kernel of the same op")
