@@ -5,8 +5,9 @@
 // in tensor memory. A tile is 256 (row, head) pairs of one sequence and one kv head, rows first: pair x is row x / G, query head x % G.
 // All heads that share the kv head ride in one tile, so the keys and values that it takes from the cache, and expands, serve G times
 // the rows, and a short chunk fills the tile. Two groups of 128 pairs take turns on the tensor core:
-//   warps 0-3 / 4-7   first the query rows to shared memory; then a thread per pair: per block of 64 keys its scores from tensor memory, masks, running maximum, weights back into
-//                     tensor memory as operand A of the next product; at the end its output row, through shared memory
+//   warps 0-3 / 4-7   first the query rows to shared memory; then a thread per pair: per block of 64 keys its scores from tensor memory,
+//                     masks, running maximum, weights back into tensor memory as operand A of the next product; at the end its output
+//                     row, through shared memory
 //   warp 8            issues S = Q K^T
 //   warp 9            issues O += P V
 //   warps 12-15       bring keys and values from their pages into the swizzled tiles that the products read: bf16 as 16-byte
@@ -15,8 +16,15 @@
 // again as soon as the threads have them in registers, so the scores of the next block are computed while the threads are at this one,
 // and the product with its weights while they are at the next; they wait for one only where their maximum makes them rescale O. (One
 // buffer of 128 scores with the weights in place: 6500 cycles for 128 keys, 2300 of them each group's wait for its two products. Two
-// buffers of 64, in place: 4200.) Products of 64 columns cost 48 cycles of the shared memory port where 128 cost 64: 2560 cycles for 128
-// keys and 256 pairs instead of 2048.
+// buffers of 64, in place: 4200.) What bounds it: the four products of 64 keys and 256 pairs are 1540 cycles of the tensor cores, a block takes
+// 2100 with bf16 pages and 2900 with e4m3 ones. The threads between the two products do (512 cycles of exponentials for each group, on the
+// same units), and with e4m3 the warps that expand the codes. Both groups on 16 warps of half a row each were slower (125 to 180 us where
+// this took 102 to 118), and so was fetching two blocks of codes ahead in registers (117 us for 105).
+//
+// Measured at 32 query heads over 8 kv heads of 128: a chunk of 512 rows behind 7500 tokens 105 us in e4m3 and 88 in bf16 pages (621 and
+// 735 TFLOP/s), 256 rows behind 16000 tokens with 37 kv heads, a tile for every SM, 450 and 344 us (694 and 911); six prompts of 200 to 2048
+// rows 104 us, 16 rows behind 4000 tokens 21.
+//
 // (A bulk tensor copy could fetch bf16 pages, but not expand codes, nor leave out single rows of a page that hold nothing yet: what
 // lies behind a sequence's last row may be NaN, and 0 * NaN would reach its sums.)
 //
@@ -25,7 +33,10 @@
 // which is that of w 2^-e. With bf16 pages the factor is the softmax scale and e is 0. Keys that a sequence has no page for have e = -infinity.
 //
 // With few tiles the keys are split too: each of `splits` CTAs takes a part of the tile's blocks and leaves O (unnormalised, 32
-// bits), M and l; a second kernel adds them up in order.
+// bits), M and l; a second kernel adds them up in order. (Dealing out equal stretches of all tiles' blocks to one CTA per SM instead, the
+// next tile's queries fetched during the last block of one, took 111 us for the 105 of the chunk and 152 for the 127 of the prompts in
+// e4m3: a change of tile costs such a CTA as much as a new one, 10,000 cycles, and the cuts come on top. Two groups that share the
+// keys of a tile of 128 pairs gained nothing below 128 pairs: there the copying warps are the bound.)
 #include "paged.cuh"
 
 #include <type_traits>
@@ -50,7 +61,9 @@ struct PagedPrefillParams {
   unsigned int* err;
 };
 
-constexpr int PP_THREADS = 512, PP_KEYS = 64, PP_JOIN = 16;
+constexpr int PP_THREADS = 512, PP_KEYS = 64;
+constexpr int PP_JOIN = 16;     // blocks of the second kernel for a tile, a pair or two per warp: 105 us for the chunk, 112 with 4
+
 template <int D, bool FP8>
 struct PagedPrefill {
   static constexpr int TILE = 128 * D * 2, KTILE = PP_KEYS * D * 2;

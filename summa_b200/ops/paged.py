@@ -31,7 +31,8 @@ class PagedRows(NamedTuple):
     """The sequences of a call. `table` `[B, P]` int32: the pages of each, in order (entries that no position of it needs may hold
     anything). `lengths` `[B]` int32: the tokens it had in the cache before the call, negative for a slot that is not in use.
     `starts` `[B + 1]` int32, ascending from 0: sequence b has the rows starts[b] .. starts[b + 1] of the call, and rows behind the last
-    belong to nobody; None: one row each. `max_rows`: the most rows of one sequence, as far as the host knows it."""
+    belong to nobody; None: one row each. `max_rows`: the most rows of one sequence, which the launch is shaped for (None: the rows of the
+    call); rows beyond it may be left out, and are reported in the error word."""
     table: torch.Tensor
     lengths: torch.Tensor
     starts: Optional[torch.Tensor] = None
@@ -104,6 +105,8 @@ def check(x: torch.Tensor, Hkv: int, D: int, kv: PagedKV, rows: PagedRows) -> La
             raise ValueError(f"{x.shape[0]} rows for {B} sequences without starts")
     elif starts.dtype != torch.int32 or starts.shape != (B + 1,) or not starts.is_contiguous() or starts.device != device:
         raise ValueError(f"starts: int32 [{B + 1}] on the device of the rows")
+    if x.shape[0] > 0 and not (B and P and pages):
+        raise ValueError(f"{x.shape[0]} rows, and a table [{B}, {P}] over {pages} pages")
     if max_rows is not None and max_rows < 1:
         raise ValueError(f"max_rows {max_rows}")
     return Layout(B, P, page, pages, table_ld, k_page, k_head, v_page, v_head, ks_ld, vs_ld)

@@ -304,6 +304,57 @@ def test_append_positions_without_a_place_store_nothing():
                 assert torch.equal(g[[0, 1, 3]], w[[0, 1, 3]]) and not torch.equal(g[2], w[2])
 
 
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows", [None, "ragged"])
+def test_append_of_many_sequences(kind, rows):
+    """Thousands of sequences of one row, and 1100 of none to five, with head counts that the heads of a thread do not divide, against the
+    plain form on the CPU: each side rounds a result once (2 * 2^-8), the rotation and its sums are off by 2^-20 of the head's size on each."""
+    D, page, Hq, Hkv = 64, 16, 5, 2
+    g = torch.Generator().manual_seed(11)
+    if rows is None:
+        held, n = torch.randint(0, 40, (5001,), generator=g).tolist(), None
+    else:
+        held, n = torch.randint(-3, 40, (1100,), generator=g).tolist(), torch.randint(0, 6, (1100,), generator=g).tolist()
+    pr, pages = _rows(held, n or [1] * len(held), page, "cpu", one=n is None)
+    kv = _cache(pages, Hkv, page, D, kind, "cpu")
+    T = sum(n) if n else len(held)
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, generator=g).to(torch.bfloat16)
+    qg, kg = 1 + 0.1 * torch.randn(D, generator=g), 1 + 0.1 * torch.randn(D, generator=g)
+    cos, sin = _table(64, D, "cpu")
+    there = _to(kv, "cuda")
+    want = ops.paged_append(qkv, qg, kg, 1e-5, cos, sin, Hq, Hkv, D, kv, pr).double()
+    got = ops.paged_append(qkv.cuda(), qg.cuda(), kg.cuda(), 1e-5, cos.cuda(), sin.cuda(), Hq, Hkv, D, there,
+                           PagedRows(*(None if t is None else t.cuda() for t in pr[:3])))
+    assert _flag() == 0
+    assert ((got.cpu().double() - want).abs() <= 2.0 ** -7 * want.abs() + 2.0 ** -19 * want.norm(dim=-1, keepdim=True)).all()
+    for x, w in ((there.k, kv.k), (there.v, kv.v)):
+        x, w = x.cpu().double(), w.double()
+        if kind == "bf16":
+            assert ((x - w).abs() <= 2.0 ** -7 * w.abs() + 2.0 ** -19 * w.norm(dim=-1, keepdim=True)).all()
+        else:
+            assert (x != w).double().mean() <= 1e-4 and ((x - w).abs() <= 2.0 ** -3 * w.abs() + 2.0 ** -9).all()
+    if kind == "e4m3":
+        assert torch.equal(there.k_scale.cpu(), kv.k_scale) and torch.equal(there.v_scale.cpu(), kv.v_scale)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_append_of_more_rows_than_promised(kind):
+    """max_rows too small: rows are stored or left as they were, the queries come back, and what was left out is reported."""
+    D, page, n = 128, 64, 50
+    pr, pages = _rows([0], [n], page, "cuda", max_rows=2)
+    kv = _cache(pages, 1, page, D, kind, "cuda")
+    old = _clone(kv)
+    qkv = torch.ones(n, 3 * D, dtype=torch.bfloat16, device="cuda")
+    q = ops.paged_append(qkv, None, None, 0.0, None, None, 1, 1, D, kv, pr)
+    flag, at = _flag(), pr.table[0, 0].item()
+    stored = (kv.v[at, 0, :n].float() * (1.0 if kind == "bf16" else kv.v_scale[at, 0].item()) == 1).all(-1)
+    kept = (kv.v[at, 0, :n].view(torch.uint8) == old.v[at, 0, :n].view(torch.uint8)).all(-1)
+    assert (q == 1).all() and stored[:2].all() and (stored | kept).all() and flag == (0 if stored.all() else 4)
+    assert torch.equal(kv.v[at, 0, n:].view(torch.uint8), old.v[at, 0, n:].view(torch.uint8))
+
+
 # ------------------------------------------------------------------ attention
 
 ATTEND = [
@@ -400,6 +451,24 @@ def test_nan_stays_in_its_sequence(kind, rows):
     got, n = ops.paged_attention(q, kv, pr), (rows or [1])[0]
     assert got[n:2 * n, :, 5].isnan().all()
     assert torch.equal(got[:n], clean[:n]) and torch.equal(got[2 * n:], clean[2 * n:]) and torch.equal(got[n:2 * n, :, :5], clean[n:2 * n, :, :5])
+
+
+@gpu
+@pytest.mark.parametrize("rows", [None, [2, 3], [50, 50]])
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_queries_that_are_not_finite(kind, rows):
+    """A NaN or an infinity in a query row makes that row of that head NaN and changes no other, to the bit."""
+    pr, pages = _rows([300, 70], rows or [1, 1], 32, "cuda", one=rows is None)
+    kv = _cache(pages, 2, 32, 128, kind, "cuda")
+    T = sum(rows) if rows else 2
+    q = torch.randn(T, 4, 128, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    want = ops.paged_attention(q, kv, pr)
+    bad = q.clone()
+    bad[0, 1, 5], bad[T - 1, 2, 127], bad[T - 1, 3, 0] = float("nan"), float("inf"), float("-inf")
+    got = ops.paged_attention(bad, kv, pr)
+    hit = torch.zeros(T, 4, dtype=torch.bool, device="cuda")
+    hit[0, 1] = hit[T - 1, 2] = hit[T - 1, 3] = True
+    assert got[hit].isnan().all() and torch.equal(got[~hit], want[~hit]) and _flag() == 0
 
 
 @gpu
@@ -683,6 +752,21 @@ def test_refusals(device):
         append(qkv=qkv.clone().requires_grad_())
     with torch.no_grad():
         attend(q=q.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_need_a_table_and_pages(device):
+    q, kv, pr = _good(device)
+    qkv = torch.randn(2, 8 * 64).to(torch.bfloat16).to(device)
+    none = PagedKV(*(t[:0] for t in kv))
+    nobody = PagedRows(pr.table[:0], pr.lengths[:0], torch.zeros(1, dtype=torch.int32, device=device))
+    for cache, rows in ((kv, pr._replace(table=pr.table[:, :0])), (none, pr), (kv, nobody)):
+        with pytest.raises(ValueError):
+            ops.paged_attention(q, cache, rows)
+        with pytest.raises(ValueError):
+            ops.paged_append(qkv, None, None, 0.0, None, None, 4, 2, 64, cache, rows)
+        # (no rows, nothing to refuse)
+        assert ops.paged_attention(q[:0], cache, rows if rows is nobody else rows._replace(starts=torch.zeros(3, dtype=torch.int32, device=device))).shape == (0, 4, 64)
 
 
 def test_bad_pages_on_the_cpu():
