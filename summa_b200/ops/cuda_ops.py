@@ -591,10 +591,11 @@ N.register("sb_paged_prefill_workspace", [N.I] * 7, restype=ctypes.c_long)
 # that as many arguments of a foreign call do.
 _PAGED_APPEND = struct.Struct("=14Q9q11if")
 _PAGED_ATTENTION = struct.Struct("=11Q11q12ifi")
-# Rows of a sequence times query heads of a kv head that the streaming kernel takes; the tiled one takes any number, 256 to a tile. At 16 the
-# streaming one is ahead at every length (us, streaming / tiled at 16 columns, e4m3: one sequence of 500 tokens 11 / 13, one of 100,003
-# 45 / 168, 64 of 4000 105 / 420; bf16 9.4 / 12, 72 / 133, 175 / 326); for more its sums would not fit its registers.
-PAGED_COLUMNS = 16
+# Rows of a sequence times query heads of a kv head, 16 at a time, that the streaming kernel takes, by the pages' element; the tiled one takes any
+# number, 256 to a tile. us, streaming / tiled: 16 columns in e4m3, one sequence of 500 tokens 11 / 13, one of 100,003 45 / 168, 64 of 4000
+# 105 / 420, in bf16 9.6 / 12, 72 / 133, 175 / 326; 32 in e4m3 11 / 13, 76 / 162, 194 / 404, in bf16 10 / 12, 133 / 128, 331 / 310; 48 in e4m3
+# 11 / 13, 104 / 163, 288 / 420, in bf16 11 / 12, 194 / 136, 491 / 325; 64 in e4m3 12 / 13, 135 / 164, 402 / 408, 64 of 500 91 / 78.
+PAGED_COLUMNS = {torch.float8_e4m3fn: 48, BF16: 32}
 
 
 def _heads_ok(t: torch.Tensor) -> bool:
@@ -663,7 +664,7 @@ def paged_attention(q, kv, rows, layout, causal=True, window=None, scale=None, o
         B, P, page, pages, table_ld, k_page, k_head, v_page, v_head, ks_ld, vs_ld = layout
         Hkv, most = k.shape[1], rows.most(T)
         G = Hq // Hkv
-        if most * G <= PAGED_COLUMNS:
+        if most * G <= PAGED_COLUMNS[k.dtype]:
             name = "sb_paged_attention"
             need = _paged_workspace(device.index, "sb_paged_attention_workspace", B, Hkv, P, page, D, 0 if ks is None else 1, most * G)
         else:

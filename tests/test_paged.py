@@ -377,7 +377,12 @@ ATTEND = [
     ([300, 0], [66, 140], 4, 1, 64, 128, True, 50),
     ([120], [18], 24, 1, 64, 16, True, None),                                 # twenty-four heads share one
     ([1200], [17], 8, 8, 128, 64, True, None),                                # keys split, one group of a tile empty
-    ([500], None, 24, 1, 128, 64, True, None),                                # one row, more columns than the streaming kernel takes
+    ([500], None, 24, 1, 128, 64, True, None),                                # one row, 24 columns
+    ([1200], [57], 8, 8, 128, 64, True, None),                                # one group of a tile empty
+    ([700, 31, 0, 1300], [5, 12, 1, 0], 8, 2, 128, 64, True, None),           # columns taken in three groups
+    ([650, 90], [8, 5], 8, 2, 64, 32, False, 37),
+    ([400, -1, 20], [7, 2, 9], 5, 1, 64, 16, True, 200),                      # rows across the groups
+    ([90], None, 48, 1, 128, 128, True, None),
 ]
 
 
@@ -552,6 +557,19 @@ def test_more_rows_than_promised():
     assert _flag() == 4 and (got[2:] == 0).all()
     want, size = _exact_attention(q, kv, pr, True, None)
     assert got[:2].isfinite().all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_more_rows_than_promised_in_groups(kind):
+    pr, pages = _rows([900, 3], [11, 2], 16, "cuda", max_rows=7)
+    kv = _cache(pages, 1, 16, 64, kind, "cuda")
+    q = torch.randn(13, 4, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    got = ops.paged_attention(q, kv, pr)
+    assert _flag() == 4 and (got[7:11] == 0).all()
+    want, size = _exact_attention(q, kv, pr, True, None)
+    _near(got[:7], want[:7], size[:7], kind == "e4m3")
+    _near(got[11:], want[11:], size[11:], kind == "e4m3")
 
 
 @gpu
