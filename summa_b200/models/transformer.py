@@ -415,6 +415,11 @@ class Transformer(nn.Module):
             live = state.paged.active()
             if not any(live):
                 live = [True] * len(live)
+                if state.pos > 0:                # all were released: recurrent states start anew with the new sequences
+                    state.pos = 0
+                    for i, blk in enumerate(self.layers):
+                        if blk.ssm is not None:
+                            state.layers[i] = blk.ssm.make_state(len(live), tokens.device, state.layers[i].conv.dtype)
             elif not all(live) and tokens.shape[1] != 1:
                 raise ValueError("some slots are not in use: bring their prompts with forward_ragged_with_state")
             if len(live) != tokens.shape[0]:
@@ -446,7 +451,10 @@ class Transformer(nn.Module):
         logits = torch.zeros(len(grow), self.cfg.vocab_size, dtype=self.stream_dtype or self.embedding.weight.dtype, device=dev)
         if not any(grow):
             return logits
-        flat = torch.cat([torch.as_tensor(p, dtype=torch.long, device=dev).reshape(-1) for p in prompts])[None]
+        ids = [torch.as_tensor(p, dtype=torch.long, device=dev) for p in prompts]
+        if any(t.dim() != 1 for t in ids):
+            raise ValueError("a prompt is one row of tokens")
+        flat = torch.cat(ids)[None]
         state.paged.begin(grow)
         x = self.embed(flat)
         rope = self.rope(dev)

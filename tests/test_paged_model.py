@@ -115,6 +115,29 @@ def test_steps_pass_over_slots_that_are_not_in_use():
             m.forward_with_state(torch.zeros(2, 1, dtype=torch.long), st)
 
 
+def test_released_sequences_leave_nothing_behind():
+    """New prompts after all slots were released, in a model with recurrent layers: as in a fresh state."""
+    cfg = mal.get_builtin_model("hybrid_tiny")
+    cfg.vocab_size = 300
+    torch.manual_seed(0)
+    m = Transformer(cfg).eval()
+    a, b = torch.randint(0, 300, (2, 2, 20))
+    with torch.no_grad():
+        st = m.make_paged_state(2, 64)
+        m.forward_with_state(a, st)
+        for slot in (0, 1):
+            st.paged.release(slot)
+        torch.testing.assert_close(m.forward_with_state(b, st), m.forward_with_state(b, m.make_paged_state(2, 64)), rtol=0, atol=0)
+
+
+def test_a_prompt_is_one_row():
+    m = _model("cpu")
+    st = m.make_paged_state(2, 64)
+    with pytest.raises(ValueError):
+        m.forward_ragged_with_state([torch.ones(1, 5, dtype=torch.long), None], st)
+    assert st.paged.held == [-1, -1] and len(st.paged.free) == st.paged.num_pages
+
+
 def test_paged_refusals():
     m = _model("cpu")
     with pytest.raises(ValueError):
