@@ -749,7 +749,9 @@ static int launch_paged_prefill(PagedPrefillParams& p, cudaStream_t st) {
 }
 
 // Tiles that T rows of B sequences can need, and parts that the keys of a tile are split into: as many as make the rounds of CTAs over
-// the GPU the shortest, a part costing two blocks of keys beside its own (a start, and its share of the join).
+// the GPU the shortest, a part costing two blocks of keys beside its own (a start, and its share of the join). A chunk of 512 rows behind 7500
+// tokens (64 tiles): 178 us whole, 106 in two parts, which is what it comes to; 16 rows behind 4000 (8 tiles): 92 whole, 52 in two,
+// 32 in four, 21 in sixteen.
 static int paged_prefill_shape(int T, int B, int Hkv, int G, long keys, int* splits) {
   const long tiles = static_cast<long>(T) * G / 256 + min(B, T);
   const long items = tiles * Hkv, blocks = (keys + 127) / 128, sms = num_sms();
