@@ -638,6 +638,9 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
         }
       }
     } else {
+      // At D = 128 a warp's rows of the stage are rows of another's queries. With keys those are at rest, since the last product is behind
+      // them; a tile without a block of keys has no product, and its four warps meet here.
+      if (nblk == 0) asm volatile("bar.sync %0, 128;" ::"r"(1 + a) : "memory");
       // (a sum of nothing: no key, zeros; a NaN stays one)
       const float inv_l = l == 0.f ? 0.f : 1.f / l;
       const long mine = pair_offset(p.o_ld, p.o_head);

@@ -717,6 +717,27 @@ def test_a_run_together(kind, device):
         assert (got.float() - want).norm() <= (0.01 if kind == "bf16" else 0.1) * want.norm()
 
 
+# ------------------------------------------------------------------ tiles without keys, tables that end
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_a_tile_without_keys_gives_zeros_whole(kind):
+    """A slot that is not in use brings more rows than half a tile has, behind a table so short that the keys are taken in one part: its
+    rows are zeros, every time, whatever its queries hold."""
+    D, page, Hq, Hkv = 128, 64, 8, 2
+    table = torch.tensor([[0, 1], [2, 3], [-1, -1]], dtype=torch.int32, device="cuda")
+    kv = _cache(4, Hkv, page, D, kind, "cuda")
+    rows = [70, 64, 101]
+    starts = torch.tensor([0] + rows).cumsum(0).to(torch.int32).cuda()
+    q = torch.randn(sum(rows), Hq, D, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    pr = PagedRows(table, torch.tensor([-1, 30, -7], dtype=torch.int32, device="cuda"), starts, max(rows))
+    want, size = _exact_attention(q, kv, pr, True, None)
+    for _ in range(50):
+        got = ops.paged_attention(q, kv, pr)
+        assert (got[:70] == 0).all() and (got[134:] == 0).all()
+        _near(got, want, size, kind == "e4m3")
+    assert _flag() == 0
+
 # ------------------------------------------------------------------ refusals
 
 def _good(device="cpu", kind="e4m3"):
