@@ -679,7 +679,8 @@ paged_decode_kernel(const PagedAttnParams p) {
         }
       }
     }
-    if (__builtin_expect(s.extra > 0 && cur.u == 0 && col0 == 0, 0)) {
+    // rows beyond the promised ones, or positions behind the table's end
+    if (__builtin_expect((s.extra > 0 || (s.len >= 0 && s.hi < static_cast<long>(s.len) + s.rows)) && cur.u == 0 && col0 == 0, 0)) {
       if (threadIdx.x == 0) atomicOr(p.err, 4u);
       for (long i = threadIdx.x; i < static_cast<long>(s.extra) * p.G * (D / 8); i += PD_WARPS * 32) {
         const long r = i / (p.G * (D / 8));

@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     }
     *abort_flag = 0;
     fence_barrier_init();
+    if (tl.hi < static_cast<long>(tl.len) + tl.rows && tl.len >= 0) atomicOr(p.err, 4u);      // positions behind the table's end
   }
   if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before();

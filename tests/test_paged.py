@@ -738,6 +738,38 @@ def test_a_tile_without_keys_gives_zeros_whole(kind):
         _near(got, want, size, kind == "e4m3")
     assert _flag() == 0
 
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows", [None, [2, 3], [6, 11], [70, 40]])
+@pytest.mark.parametrize("window", [None, 40])
+def test_a_table_that_ends_before_its_sequence(window, rows, kind):
+    """The last positions of a sequence have no place in the table: bit 4 of the error word, and rows as if those keys were not there. The
+    other sequence is served."""
+    D, page, Hq, Hkv = 64, 16, 4, 1
+    n = rows or [1, 1]
+    pr, pages = _rows([20, 95], n, page, "cuda", one=rows is None, spare=0, max_rows=max(n))
+    kv = _cache(pages, Hkv, page, D, kind, "cuda")
+    q = torch.randn(sum(n), Hq, D, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
+    want, size = _exact_attention(q, kv, pr, True, window)
+    _near(ops.paged_attention(q, kv, pr, True, window), want, size, kind == "e4m3")
+    assert _flag() == 0                                                  # (as wide as it has to be)
+    cut = pr._replace(table=pr.table[:, :-1].contiguous())
+    got = ops.paged_attention(q, kv, cut, True, window)
+    assert _flag() == 4
+    _near(got[:n[0]], want[:n[0]], size[:n[0]], kind == "e4m3")
+    there = max(0, cut.table.shape[1] * page - 95)                       # rows of the second sequence whose keys all have a place
+    if there:
+        _near(got[n[0]:n[0] + there], want[n[0]:n[0] + there], size[n[0]:n[0] + there], kind == "e4m3")
+    assert got.isfinite().all()
+
+
+@pytest.mark.parametrize("rows", [None, [2, 3]])
+def test_a_table_that_ends_is_an_error_on_the_cpu(rows):
+    pr, pages = _rows([20, 95], rows or [1, 1], 16, "cpu", one=rows is None, spare=0)
+    kv = _cache(pages, 1, 16, 64, "bf16", "cpu")
+    with pytest.raises(RuntimeError, match="no page"):
+        ops.paged_attention(torch.zeros(sum(rows or [1, 1]), 4, 64, dtype=torch.bfloat16), kv, pr._replace(table=pr.table[:, :-1]))
+
 # ------------------------------------------------------------------ refusals
 
 def _good(device="cpu", kind="e4m3"):
