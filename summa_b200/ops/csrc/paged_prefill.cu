@@ -39,8 +39,6 @@
 // keys of a tile of 128 pairs gained nothing below 128 pairs: there the copying warps are the bound.)
 #include "paged.cuh"
 
-#include <type_traits>
-
 namespace sb {
 
 struct PagedPrefillParams {
@@ -487,7 +485,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       khi = static_cast<int>(min(static_cast<long>(khi), pos + p.window + 1));
     }
     if (!live) khi = 0;
-    float m_ref = -INFINITY, l = 0.f;
+    float m_ref = -INFINITY, l = 0.f, top_e = -INFINITY;          // top_e: the largest exponent of a page's scale so far
     bool ok = a < tiles_here;
 #pragma unroll 1
     for (int i = 0; i < nblk && ok; ++i) {
@@ -531,7 +529,11 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       const bool grow = m_blk > m_ref + C::SLACK;
       if (__any_sync(0xffffffffu, grow)) {
         const float m_new = grow ? m_blk : m_ref;
-        const float alpha = grow ? (m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m_new)) : 1.f;
+        const float half = !grow ? 1.f : m_ref == -INFINITY ? 0.f : FP8 ? exp2_half(m_ref, m_new) : fast_exp2(m_ref - m_new);
+        const float alpha = FP8 ? half * half : half;
+        l *= half;
+        if (FP8) l *= half;
+        m_ref = m_new;
         if (i > 0) {
           // O is at rest once the product of the block before is complete: this block's waits for its weights
           if (!mbar_wait(&o_full[a * 2 + (b ^ 1)], ((i - 1) >> 1) & 1, abort_flag, p.err)) { ok = false; break; }
@@ -546,8 +548,6 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
             tmem_st_32x32b_x16(t_o + cc * 16, o16);
           }
         }
-        l *= alpha;
-        m_ref = m_new;
       }
       // this buffer's weights of two blocks ago have been used
       if (i > 1) {
@@ -555,52 +555,45 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
         tc_fence_after();
       }
       const float nm = C::HEAD - (m_ref == -INFINITY ? 0.f : m_ref);
-      // (of pages far apart in scale the one's w is nothing beside the other's, its share of l is not: where a page is 2^80 below, l comes
-      // from the scores)
-      bool apart = false;
+      if (FP8) {
+        // Of pages far apart in scale the one's w is nothing beside the other's, its share of l is not: behind a page 2^100 above, l comes from
+        // the scores. Short of that a share down to 2^-25 of the largest has a w of 2^(e - the largest e - 16) or more, which 32 bits hold.
+        top_e = fmaxf(fmaxf(top_e, fmaxf(e[0], e[1])), fmaxf(e[2], e[3]));
+        if (__builtin_expect(fminf(fminf(e[0], e[1]), fminf(e[2], e[3])) + 100.f < top_e, 0)) {
 #pragma unroll
-      for (int gp = 0; gp < 4; ++gp) apart |= FP8 && e[gp] + nm < -80.f;
-      auto weights = [&](auto far) {
-        constexpr bool FAR = decltype(far)::value;
+          for (int k = 0; k < 64; ++k) l += inv[k >> 4] != 0.f ? fast_exp2(fmaf(__uint_as_float(v[k]), fs[k >> 4], nm)) : 0.f;
+          inv[0] = inv[1] = inv[2] = inv[3] = 0.f;
+        }
+      }
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          uint32_t pk[16];
+      for (int cc = 0; cc < 2; ++cc) {
+        uint32_t pk[16];
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            const int gp = cc * 2 + hh;
-            const float n1 = FP8 ? e[gp] + nm : nm;
-            const uint64_t f2 = f2_pack(fs[gp], fs[gp]), n2 = f2_pack(n1, n1);
-            uint64_t sum2 = f2_pack(0.f, 0.f);
+        for (int hh = 0; hh < 2; ++hh) {
+          const int gp = cc * 2 + hh;
+          const float n1 = FP8 ? e[gp] + nm : nm;
+          const uint64_t f2 = f2_pack(fs[gp], fs[gp]), n2 = f2_pack(n1, n1);
+          uint64_t sum2 = f2_pack(0.f, 0.f);
 #pragma unroll
-            for (int jj = 0; jj < 8; ++jj) {
-              const int k = gp * 16 + 2 * jj;
-              float y0, y1;
-              f2_unpack(f2_fma(f2_pack_u(v[k], v[k + 1]), f2, n2), y0, y1);
-              const float e0 = fast_exp2(y0), e1 = fast_exp2(y1);
-              sum2 = f2_add(sum2, f2_pack(e0, e1));
-              if (FP8) {
-                const __half2 h = __floats2half2_rn(e0, e1);
-                pk[hh * 8 + jj] = *reinterpret_cast<const uint32_t*>(&h);
-              } else {
-                pk[hh * 8 + jj] = pack_bf16(e0, e1);
-              }
-            }
-            float s0, s1;
-            f2_unpack(sum2, s0, s1);
-            if (FAR) {
-              if (inv[gp] != 0.f) {
-#pragma unroll
-                for (int k = gp * 16; k < gp * 16 + 16; ++k) l += fast_exp2(fmaf(__uint_as_float(v[k]), fs[gp], nm));
-              }
+          for (int jj = 0; jj < 8; ++jj) {
+            const int k = gp * 16 + 2 * jj;
+            float y0, y1;
+            f2_unpack(f2_fma(f2_pack_u(v[k], v[k + 1]), f2, n2), y0, y1);
+            const float e0 = fast_exp2(y0), e1 = fast_exp2(y1);
+            sum2 = f2_add(sum2, f2_pack(e0, e1));
+            if (FP8) {
+              const __half2 h = __floats2half2_rn(e0, e1);
+              pk[hh * 8 + jj] = *reinterpret_cast<const uint32_t*>(&h);
             } else {
-              l = FP8 ? fmaf(s0 + s1, inv[gp], l) : l + (s0 + s1);
+              pk[hh * 8 + jj] = pack_bf16(e0, e1);
             }
           }
-          tmem_st_32x32b_x16(tmem_base + C::COL_P + (a * 2 + b) * 32 + lane_sel + cc * 16, pk);
+          float s0, s1;
+          f2_unpack(sum2, s0, s1);
+          l = FP8 ? fmaf(s0 + s1, inv[gp], l) : l + (s0 + s1);
         }
-      };
-      if (FP8 && __any_sync(0xffffffffu, apart)) weights(std::integral_constant<bool, FP8>{});
-      else weights(std::false_type{});
+        tmem_st_32x32b_x16(tmem_base + C::COL_P + (a * 2 + b) * 32 + lane_sel + cc * 16, pk);
+      }
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&p_full[a * 2 + b]);
@@ -702,8 +695,8 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PagedPref
     for (int s = 0; s < p.splits; ++s) {
       const float2 w = *reinterpret_cast<const float2*>(ml0 + (s * stride + at) * 2);
       if (w.x == -INFINITY && w.y == 0.f) continue;      // no key there: its O was not written
-      const float f = w.x == -INFINITY ? 0.f : fast_exp2(w.x - top);
-      sum += w.y * f;
+      const float half = w.x == -INFINITY ? 0.f : exp2_half(w.x, top), f = half * half;
+      sum += w.y * half * half;
       const float* y = p.part + (s * stride + at) * D + lane * V;
       if (V == 4) {
         const float4 z = *reinterpret_cast<const float4*>(y);

@@ -770,6 +770,35 @@ def test_a_table_that_ends_is_an_error_on_the_cpu(rows):
     with pytest.raises(RuntimeError, match="no page"):
         ops.paged_attention(torch.zeros(sum(rows or [1, 1]), 4, 64, dtype=torch.bfloat16), kv, pr._replace(table=pr.table[:, :-1]))
 
+@gpu
+@pytest.mark.parametrize("rows", [None, [4], [9], [40]])
+@pytest.mark.parametrize("order", ["up", "down", "inside", "far back"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_value_scales_that_leave_the_weights_apart(D, order, rows):
+    """Pages whose value scales are 2^170 apart: all scores alike; and all of them below -64, the small pages' 8 above or below the large
+    ones'. Every key counts in the sum of the weights, whatever the scale of its page."""
+    page, Hq = 16, 4
+    g = torch.Generator().manual_seed(6)
+    n = (rows or [1])[0]
+    held = 5000 if order == "far back" else 800
+    pr, pages = _rows([held], [n], page, "cuda", one=rows is None, max_rows=n)
+    kv = _cache(pages, 1, page, D, "e4m3", "cuda", seed=1)
+    ids = pr.table[0, :-(-(held + n) // page)].long()
+    i = torch.arange(len(ids), device="cuda")
+    small = {"up": i < len(ids) // 2, "down": i >= len(ids) // 2, "inside": i % 2 == 0, "far back": i < 280}[order]
+    kv.v_scale[ids, 0] = torch.where(small, 2.0 ** -60, 2.0 ** 110)
+    kv.k[...] = (torch.randn(kv.k.shape, generator=g) / 4).to(E4M3).cuda()
+    kv.k_scale.fill_(1.0)
+    q = torch.randn(n, Hq, D, generator=g).to(torch.bfloat16).cuda()
+    want, size = _exact_attention(q, kv, pr, True, None)
+    _near(ops.paged_attention(q, kv, pr), want, size, True)
+    q[..., 0] = 8.0 if D == 64 else 11.3125                              # the first dimension of a key is its score, but for the noise of the others
+    for low, high in ((-64.0, -72.0), (-72.0, -64.0)):
+        kv.k[ids, 0, :, 0] = torch.where(small, low, high)[:, None].to(E4M3)
+        want, size = _exact_attention(q, kv, pr, True, None)
+        _near(ops.paged_attention(q, kv, pr), want, size, True)
+    assert _flag() == 0
+
 # ------------------------------------------------------------------ refusals
 
 def _good(device="cpu", kind="e4m3"):
