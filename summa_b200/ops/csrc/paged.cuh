@@ -96,6 +96,9 @@ __device__ __forceinline__ int e4m3_exp(float most) {
 
 // With 8-bit values a sum of weights l is taken against a maximum of s + e, not of s, so where the scales of two pages lie 2^126 or more apart
 // a factor 2^d that brings l to another maximum may be below what 32 bits hold while l 2^d is not. It comes as two halves (e spans 180).
+// And l is held 2^PAGED_SUM times as large: under scales of 2^120 the share of a key far below the largest, which many of them make count,
+// would otherwise be less than 32 bits hold.
+constexpr int PAGED_SUM = 20;
 __device__ __forceinline__ float exp2_half(float from, float to) { return fast_exp2(0.5f * from - 0.5f * to); }
 
 // Two values to two e4m3 codes (the first in the low byte): nearest, ties to even, NaN for NaN. Infinities come as NaN from the

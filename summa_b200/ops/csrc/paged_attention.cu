@@ -260,7 +260,7 @@ paged_decode_kernel(const PagedAttnParams p) {
   constexpr int NS = PD_NS, KT = C::KT, MT = C::MT, UNIT = C::UNIT, ROW = C::ROW, COLS = 8 * NT, MD = D / 16, KSTEPS = D / 16;
   constexpr int RB = NT == 1 ? 2 : 1;                    // warps that put their O down at a time (two CTAs have to fit an SM)
   constexpr int QUADS = NT * MD;                         // accumulators of a thread, in fours
-  constexpr float HEAD = FP8 ? 11.f : 0.f, SLACK = FP8 ? 4.f : 8.f;
+  constexpr float HEAD = FP8 ? 11.f : 0.f, SLACK = FP8 ? 4.f : 8.f, SUM = FP8 ? PAGED_SUM : 0.f;
   extern __shared__ __align__(128) uint8_t smem[];
   // Nothing is read before the wait, and the joining kernel, which reads the batch's description before its own, starts after it.
   asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
@@ -553,7 +553,7 @@ paged_decode_kernel(const PagedAttnParams p) {
           const float w0 = fast_exp2(sc[n][m][0] - r0), w1 = fast_exp2(sc[n][m][1] - r1);
           const float w2 = fast_exp2(sc[n][m][2] - r0), w3 = fast_exp2(sc[n][m][3] - r1);
           // (from the scores, not as w 2^-e: of pages 2^120 apart the one's w is nothing beside the other's, its share of l is not)
-          const float q0 = r0 + ve[m], q1 = r1 + ve[m];
+          const float q0 = r0 - SUM + ve[m], q1 = r1 - SUM + ve[m];
           l[n][0] += FP8 ? fast_exp2(sc[n][m][0] - q0) + fast_exp2(sc[n][m][2] - q0) : w0 + w2;
           l[n][1] += FP8 ? fast_exp2(sc[n][m][1] - q1) + fast_exp2(sc[n][m][3] - q1) : w1 + w3;
           pf[n][m][0] = transpose8x8(FP8 ? pack_f16(w0, w1) : pack_bf16(w0, w1));
@@ -678,7 +678,7 @@ paged_decode_kernel(const PagedAttnParams p) {
           if (i % MD == 0 && g == 0) part_ml[col] = make_float2(tp, sum);
         } else if (col0 + col < cols) {
           // (a sum of nothing: no key, zeros; a NaN stays one)
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          const float inv = sum == 0.f ? 0.f : (FP8 ? 1 << PAGED_SUM : 1) / sum;
           const int c = col0 + col;
           const long to = (s.row0 + c / p.G) * p.o_ld + (cur.kh * p.G + c % p.G) * p.o_head + paged_dim<D, FP8>(g, i % MD);
           *reinterpret_cast<uint32_t*>(p.o + to) = h ? pack_bf16(o.y * inv, o.w * inv) : pack_bf16(o.x * inv, o.z * inv);
@@ -794,7 +794,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32, 3) paged_join_kernel(const Page
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int c = col0 + 2 * pair + h;
-      const float l = h ? l1 : l0, inv = l == 0.f ? 0.f : 1.f / l;
+      const float l = h ? l1 : l0, inv = l == 0.f ? 0.f : (FP8 ? 1 << PAGED_SUM : 1) / l;
       if (c < s.rows * p.G)
         *reinterpret_cast<uint32_t*>(p.o + (s.row0 + c / p.G) * p.o_ld + (kh * p.G + c % p.G) * p.o_head + d) =
             h ? pack_bf16(o.y * inv, o.w * inv) : pack_bf16(o.x * inv, o.z * inv);

@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
   uint64_t* v_empty = bars + 25;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float4* scales = reinterpret_cast<float4*>(smem + C::OFF_SCALE);       // [RING][4]: key factor, e, 2^-e
+  float4* scales = reinterpret_cast<float4*>(smem + C::OFF_SCALE);       // [RING][4]: key factor, e, 2^(PAGED_SUM - e)
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kh = blockIdx.x;
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
         float4 f = scale;
         if (FP8) {
           const int e = min(max(scale_exp(scale.y), PAGED_LEAST_EXP), PAGED_MOST_EXP);
-          f = f.z != 0.f ? make_float4(scale.x, static_cast<float>(e), exp_scale(-e), 0.f) : make_float4(1.f, 0.f, 0.f, 0.f);
+          f = f.z != 0.f ? make_float4(scale.x, static_cast<float>(e), exp_scale(PAGED_SUM - e), 0.f) : make_float4(1.f, 0.f, 0.f, 0.f);
         }
         scales[(i % C::RING) * 4 + tid] = f;
       }
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
         top_e = fmaxf(fmaxf(top_e, fmaxf(e[0], e[1])), fmaxf(e[2], e[3]));
         if (__builtin_expect(fminf(fminf(e[0], e[1]), fminf(e[2], e[3])) + 100.f < top_e, 0)) {
 #pragma unroll
-          for (int k = 0; k < 64; ++k) l += inv[k >> 4] != 0.f ? fast_exp2(fmaf(__uint_as_float(v[k]), fs[k >> 4], nm)) : 0.f;
+          for (int k = 0; k < 64; ++k) l += inv[k >> 4] != 0.f ? fast_exp2(fmaf(__uint_as_float(v[k]), fs[k >> 4], nm + PAGED_SUM)) : 0.f;
           inv[0] = inv[1] = inv[2] = inv[3] = 0.f;
         }
       }
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       // them; a tile without a block of keys has no product, and its four warps meet here.
       if (nblk == 0) asm volatile("bar.sync %0, 128;" ::"r"(1 + a) : "memory");
       // (a sum of nothing: no key, zeros; a NaN stays one)
-      const float inv_l = l == 0.f ? 0.f : 1.f / l;
+      const float inv_l = l == 0.f ? 0.f : (FP8 ? 1 << PAGED_SUM : 1) / l;
       const long mine = pair_offset(p.o_ld, p.o_head);
 #pragma unroll 1
       for (int cc = 0; cc < D / 16; ++cc) {
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PagedPref
         o[0] += z.x * f; o[1] += z.y * f;
       }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = sum == 0.f ? 0.f : (p.ks != nullptr ? 1 << PAGED_SUM : 1) / sum;
     __nv_bfloat16* dst = p.o + (tl.row0 + (x0 + r) / G) * p.o_ld + (kh * G + (x0 + r) % G) * p.o_head + lane * V;
     if (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2 % V] * inv, o[3 % V] * inv));
     else *reinterpret_cast<uint32_t*>(dst) = pack_bf16(o[0] * inv, o[1] * inv);

@@ -799,6 +799,28 @@ def test_value_scales_that_leave_the_weights_apart(D, order, rows):
         _near(ops.paged_attention(q, kv, pr), want, size, True)
     assert _flag() == 0
 
+@gpu
+@pytest.mark.parametrize("n", [1, 4, 20])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_small_weights_under_the_largest_scale(D, n):
+    """Value scales of 2^120, one key of weight e^12 (2^17.3) among 100,000 others of 1: together they are more than a third of the sum. So
+    many sequences, all over the same pages and with the same queries, that nothing is split."""
+    page, Hq, held, B = 128, 4, 100003, 300
+    one, pages = _rows([held], [n], page, "cuda", max_rows=n)
+    kv = _cache(pages, 1, page, D, "e4m3", "cuda")
+    for t, x in zip(kv, (0.0, 0.0, 1.0, 2.0 ** 120)):
+        t.fill_(x)
+    kv.v[...] = torch.randint(1, 129, kv.v.shape, generator=torch.Generator().manual_seed(8)).to(E4M3).cuda()
+    kv.k[int(one.table[0, 300]), 0, 7, 0] = 96.0
+    q = torch.zeros(n, Hq, D, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 1.0 if D == 64 else 1.4140625
+    want, size = _exact_attention(q, kv, one, True, None)
+    starts = None if n == 1 else torch.arange(B + 1, dtype=torch.int32, device="cuda") * n
+    rows = PagedRows(one.table.expand(B, -1).contiguous(), one.lengths.expand(B).contiguous(), starts, n)
+    got = ops.paged_attention(q.repeat(B, 1, 1), kv, rows)
+    _near(got, want.repeat(B, 1, 1), size.repeat(B, 1, 1), True)
+    assert _flag() == 0
+
 # ------------------------------------------------------------------ refusals
 
 def _good(device="cpu", kind="e4m3"):
