@@ -431,7 +431,7 @@ paged_decode_kernel(const PagedAttnParams p) {
     // keys that every column sees
     const int all_lo = p.window >= 0 ? static_cast<int>(max(static_cast<long>(s.len) + s.rows - 1 - p.window, 0L)) : 0;
     const int all_hi = p.causal ? static_cast<int>(min(static_cast<long>(s.hi), s.len + 1L))
-                                : p.window >= 0 ? static_cast<int>(min(static_cast<long>(s.hi), s.len + p.window + 1L)) : s.hi;
+                                : p.window >= 0 ? static_cast<int>(min(static_cast<long>(s.hi), static_cast<long>(s.len) + p.window + 1)) : s.hi;
 
     float acc[NT][MD][4], M[NT][2], l[NT][2];
 #pragma unroll

@@ -821,6 +821,18 @@ def test_many_small_weights_under_the_largest_scale(D, n):
     _near(got, want.repeat(B, 1, 1), size.repeat(B, 1, 1), True)
     assert _flag() == 0
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows", [None, [2, 3], [70, 40]])
+def test_a_window_wider_than_32_bits_hold_hides_nothing(rows, device):
+    pr, pages = _rows([400, 37], rows or [1, 1], 16, device, one=rows is None, max_rows=max(rows or [1]))
+    for kind in ("bf16", "e4m3"):
+        kv = _cache(pages, 2, 16, 64, kind, device)
+        q = torch.randn(sum(rows or [1, 1]), 4, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(device)
+        for causal in (True, False):
+            want = ops.paged_attention(q, kv, pr, causal)
+            for window in (2 ** 31 - 2, 2 ** 31 - 1, 2 ** 31, 2 ** 40):
+                assert torch.equal(ops.paged_attention(q, kv, pr, causal, window), want)
+
 # ------------------------------------------------------------------ refusals
 
 def _good(device="cpu", kind="e4m3"):
