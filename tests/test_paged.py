@@ -921,3 +921,30 @@ def test_no_rows_is_no_work():
         none = pr._replace(starts=torch.zeros(3, dtype=torch.int32, device=device))
         assert ops.paged_attention(q[:0], kv, none).shape == (0, 4, 64)
         assert ops.paged_append(torch.zeros(0, 8 * 64, dtype=torch.bfloat16, device=device), None, None, 0.0, None, None, 4, 2, 64, kv, none).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_a_tangent_is_refused_not_dropped(kind, device):
+    import torch.autograd.forward_ad as fwd
+    q, kv, pr = _good(device, kind)
+    qkv = torch.randn(2, 8 * 64).to(torch.bfloat16).to(device)
+    gain = torch.ones(64, device=device)
+
+    def append(x=qkv, qg=gain, kg=gain):
+        return ops.paged_append(x, qg, kg, 1e-5, None, None, 4, 2, 64, kv, pr)
+
+    def dual(t):
+        return fwd.make_dual(t, torch.ones_like(t))
+
+    want = ops.paged_attention(q, kv, pr)
+    with fwd.dual_level():
+        for call in (lambda: ops.paged_attention(dual(q), kv, pr), lambda: append(dual(qkv)), lambda: append(qg=dual(gain)), lambda: append(kg=dual(gain))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert torch.equal(ops.paged_attention(q, kv, pr), want)         # without a tangent, nothing to refuse
+        append()
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda x: ops.paged_attention(x, kv, pr), (q,), (torch.ones_like(q),))
