@@ -948,3 +948,38 @@ def test_a_tangent_is_refused_not_dropped(kind, device):
         append()
     with pytest.raises(RuntimeError, match="forward-mode"):
         torch.func.jvp(lambda x: ops.paged_attention(x, kv, pr), (q,), (torch.ones_like(q),))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_no_input_drops_a_gradient(kind, device):
+    """Pages, their scales, the rotation's table and the output are refused with a gradient or a tangent like the rows are."""
+    import torch.autograd.forward_ad as fwd
+    q, kv, pr = _good(device, kind)
+    qkv = torch.randn(2, 8 * 64).to(torch.bfloat16).to(device)
+    cos, sin = _table(64, 64, device)
+
+    def attend(kv=kv, out=None):
+        return ops.paged_attention(q, kv, pr, out=out)
+
+    def append(kv=kv, cos=cos, sin=sin, out=None):
+        return ops.paged_append(qkv, None, None, 0.0, cos, sin, 4, 2, 64, kv, pr, out)
+
+    def leaf(t):
+        return t.clone().requires_grad_()
+
+    pages = ("k", "v") if kind == "bf16" else ("k_scale", "v_scale")
+    for wrap, match in ((leaf, "no_grad"), (lambda t: fwd.make_dual(t, torch.ones_like(t)), "forward-mode")):
+        with fwd.dual_level():
+            for call in (attend, append):
+                for name in pages:
+                    with pytest.raises(RuntimeError, match=match):
+                        call(kv=kv._replace(**{name: wrap(getattr(kv, name))}))
+                with pytest.raises(RuntimeError, match=match):
+                    call(out=wrap(torch.zeros_like(q)))
+            for more in ({"cos": wrap(cos)}, {"sin": wrap(sin)}):
+                with pytest.raises(RuntimeError, match=match):
+                    append(**more)
+    with torch.no_grad():                                                # (a gradient that nobody asks for is none)
+        want = attend()
+        assert torch.equal(attend(kv=kv._replace(**{n: leaf(getattr(kv, n)) for n in pages})), want)
