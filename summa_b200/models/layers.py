@@ -123,7 +123,6 @@ class MultiHeadAttention(nn.Module):
         """Attention over a fused `[B, S, q_dim + 2 kv_dim]` projection; returns `[B, S, q_dim]`
         (everything between the two projections, so tensor-parallel runners can supply their own)."""
         B, S, _ = qkv.shape
-        offset = state.length if isinstance(state, AttentionState) else 0
         cos, sin = rope if (self.use_rope and rope is not None) else (None, None)
         qg = self.q_norm.gamma if self.q_norm is not None else None
         kg = self.k_norm.gamma if self.k_norm is not None else None
@@ -132,6 +131,7 @@ class MultiHeadAttention(nn.Module):
             q = ops.paged_append(qkv.reshape(B * S, -1), qg, kg, self.eps, cos, sin, self.num_heads, self.num_kv_heads, self.head_dim,
                                  state.kv, rows)
             return ops.paged_attention(q, state.kv, rows, self.causal, self.window).reshape(B, S, self.q_dim)
+        offset = state.length if state is not None else 0
         if (state is None and ops.native_enabled(qkv) and self.head_dim in (64, 128)
                 and cos is not None and not (self.dropout > 0.0 and self.training)):
             # packed path: RoPE/QK-norm and attention run straight on the fused activation

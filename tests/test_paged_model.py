@@ -164,6 +164,17 @@ def test_paged_refusals():
         eng.decode(torch.zeros(2, 1, dtype=torch.long), 1)
 
 
+def test_a_state_of_ones_own_keeps_its_length():
+    """Whatever has `k`, `v` and `length` is a contiguous state, not `AttentionState` alone."""
+    from types import SimpleNamespace
+    m = _model("cpu")
+    tok = torch.randint(0, 500, (2, 30), generator=torch.Generator().manual_seed(0))
+    with torch.no_grad():
+        a, b = m.make_state(2, 64), m.make_state(2, 64)
+        b.layers = [SimpleNamespace(k=st.k, v=st.v, length=0) for st in b.layers]
+        for i, j in ((0, 12), (12, 13), (13, 30)):
+            assert torch.equal(m.forward_with_state(tok[:, i:j], b), m.forward_with_state(tok[:, i:j], a))
+
 # ------------------------------------------------------------------ engine and generator
 
 @pytest.mark.parametrize("kind", KINDS)
