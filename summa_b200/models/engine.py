@@ -351,7 +351,7 @@ class _GraphDecoder:
     def run(self, first: torch.Tensor, steps: int) -> torch.Tensor:
         if self.paged is not None:
             live = [int(on) for on in self.paged.active()]
-            self.paged.reserve([steps * on for on in live])
+            self.paged.take([steps * on for on in live])
             self.live.copy_(torch.tensor(live, dtype=torch.int32))
             start = self.state.pos
         else:
@@ -365,15 +365,20 @@ class _GraphDecoder:
         self.pos.fill_(start - 1)                         # the step's first kernel moves both on
         self.col.fill_(-1)
         done = 0
-        if self.graph is None:
-            allocated = "allocated_bytes.all.allocated"
-            before = torch.cuda.memory_stats().get(allocated, 0)
-            self._step()                                  # eager: warms every lazy allocation and attribute
-            done = 1
-            if steps > 1:
-                self._capture(torch.cuda.memory_stats().get(allocated, 0) - before)
-        for _ in range(steps - done):
-            self.graph.replay()
+        try:
+            if self.graph is None:
+                allocated = "allocated_bytes.all.allocated"
+                before = torch.cuda.memory_stats().get(allocated, 0)
+                self._step()                              # eager: warms every lazy allocation and attribute
+                done = 1
+                if steps > 1:
+                    self._capture(torch.cuda.memory_stats().get(allocated, 0) - before)
+            for _ in range(steps - done):
+                self.graph.replay()
+        except BaseException:
+            if self.paged is not None:                    # steps that ran moved the lengths on
+                self.paged.cancel()
+            raise
         if self.paged is not None:
             self.paged.advance([steps * on for on in live], on_device=False)
         else:

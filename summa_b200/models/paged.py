@@ -45,6 +45,8 @@ class PagedCache:
         self.pages: List[List[int]] = [[] for _ in range(batch)]
         self.free = list(range(self.num_pages - 1, -1, -1))
         self.rows: Optional[ops.PagedRows] = None        # of the forward pass under way
+        self.fresh: List[int] = []                       # slots that it takes into use, and how many pages it took for each slot
+        self.taken = [0] * batch
 
     def layer(self, kv_heads: int, head_dim: int, dtype: torch.dtype, kind: str) -> PagedAttentionState:
         dev = self.table.device
@@ -61,9 +63,9 @@ class PagedCache:
     def active(self) -> List[bool]:
         return [h >= 0 for h in self.held]
 
-    def reserve(self, grow: Sequence[int]) -> None:
+    def reserve(self, grow: Sequence[int]) -> List[int]:
         """Pages for `grow[b]` more tokens of each slot (a slot that is not in use begins with them). All of them or, where the pool or
-        a slot's capacity does not reach, none."""
+        a slot's capacity does not reach, none. Returns how many each slot took."""
         if len(grow) != self.batch or any(n < 0 for n in grow):
             raise ValueError(f"{list(grow)} more tokens for {self.batch} slots")
         need = []
@@ -75,7 +77,7 @@ class PagedCache:
         if sum(need) > len(self.free):
             raise RuntimeError(f"KV cache overflow: {sum(need)} more pages, and {len(self.free)} of {self.num_pages} are free")
         if not any(need):
-            return
+            return need
         at, ids = [], []
         for b, n in enumerate(need):
             for _ in range(n):
@@ -84,11 +86,17 @@ class PagedCache:
                 ids.append(self.pages[b][-1])
         dev = self.table.device
         self.table.view(-1)[torch.tensor(at, device=dev)] = torch.tensor(ids, dtype=torch.int32, device=dev)
+        return need
+
+    def take(self, grow: Sequence[int]) -> None:
+        """`reserve` for a forward pass: `cancel` gives these pages back."""
+        self.taken = [a + n for a, n in zip(self.taken, self.reserve(grow))]
 
     def begin(self, grow: Sequence[int]) -> ops.PagedRows:
-        """Describes a forward pass that brings `grow[b]` rows to slot b, and has pages ready for them."""
-        self.reserve(grow)
+        """Describes a forward pass that brings `grow[b]` rows to slot b, and has pages ready for them. It ends with `advance`, or with `cancel`."""
+        self.take(grow)
         fresh = [b for b, n in enumerate(grow) if n and self.held[b] < 0]
+        self.fresh += fresh
         if fresh:
             self.lengths[torch.tensor(fresh, device=self.lengths.device)] = 0
             for b in fresh:
@@ -104,23 +112,42 @@ class PagedCache:
 
     def begin_step(self, grow: Sequence[int]) -> ops.PagedRows:
         """Describes a step of one row for every slot, of which those that are not in use store nothing."""
-        self.reserve(grow)
+        self.take(grow)
         self.rows = ops.PagedRows(self.table, self.lengths)
         return self.rows
 
     def advance(self, grow: Sequence[int], on_device: bool = True) -> None:
         """The rows of the pass are in the cache. `on_device`: `lengths` too is moved on here."""
-        self.rows = None
+        self._close()
         if on_device:
             self.lengths.add_(torch.tensor(list(grow), dtype=torch.int32, device=self.lengths.device))
         self.held = [h + n if n else h for h, n in zip(self.held, grow)]
+
+    def cancel(self) -> None:
+        """The pass that was begun did not come to its end: slots have the lengths of before it, those that it took into use are out of it
+        again, and the pages that it took are free. (Rows that it has put behind a sequence are not read. In 8 bits they may have raised the
+        scale of its last page, and so have rounded that page's codes once more.)"""
+        for b, n in reversed(list(enumerate(self.taken))):       # (in the reverse of the order in which they were taken)
+            keep = len(self.pages[b]) - n
+            if n:
+                self.free.extend(reversed(self.pages[b][keep:]))
+                del self.pages[b][keep:]
+                self.table[b, keep:] = -1
+        for b in self.fresh:
+            self.held[b] = -1
+        self._close()
+        self.lengths.copy_(torch.tensor(self.held, dtype=torch.int32))
+
+    def _close(self) -> None:
+        self.rows, self.fresh, self.taken = None, [], [0] * self.batch
 
     def release(self, slot: int) -> None:
         """Takes a slot out of use; its pages go back to the pool."""
         if not 0 <= slot < self.batch:
             raise ValueError(f"slot {slot} of {self.batch}")
         self.free.extend(reversed(self.pages[slot]))
-        self.pages[slot] = []
+        self.pages[slot], self.taken[slot] = [], 0
+        self.fresh = [b for b in self.fresh if b != slot]
         self.held[slot] = -1
         self.lengths[slot] = -1
         self.table[slot] = -1

@@ -10,6 +10,7 @@ attention block.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence, Tuple
@@ -408,9 +409,24 @@ class Transformer(nn.Module):
                 layers.append(cache.layer(blk.attention.num_kv_heads, blk.attention.head_dim, dtype, kv_cache))
         return InferenceState(layers, 0, capacity, cache)
 
+    @contextlib.contextmanager
+    def _paged_pass(self, state: InferenceState, grow: Sequence[int], step: bool = False):
+        """A forward pass that brings `grow[b]` rows to slot b of a paged state (`step`: one for every slot). One that fails leaves the slots
+        and the recurrent layers as they were."""
+        recurrent = [(st, st.conv, st.h) for st in state.layers if isinstance(st, MambaState)]
+        try:
+            state.paged.begin_step(grow) if step else state.paged.begin(grow)
+            yield
+        except BaseException:
+            for st, conv, h in recurrent:
+                st.conv, st.h = conv, h
+            state.paged.cancel()
+            raise
+        state.paged.advance(grow)
+
     def forward_hidden_with_state(self, tokens: torch.Tensor, state: InferenceState) -> torch.Tensor:
         """Over a paged state (no gradients) the rows go to the slots in use, or to all where none is yet."""
-        grow = None
+        held = contextlib.nullcontext()
         if state.paged is not None:
             live = state.paged.active()
             if not any(live):
@@ -425,13 +441,12 @@ class Transformer(nn.Module):
             if len(live) != tokens.shape[0]:
                 raise ValueError(f"{tokens.shape[0]} rows for a state of {len(live)} slots")
             grow = [tokens.shape[1] if on else 0 for on in live]
-            state.paged.begin(grow) if all(live) else state.paged.begin_step(grow)
-        x = self.embed(tokens)
-        rope = self.rope(tokens.device)
-        for blk, st in zip(self.layers, state.layers):
-            x, _ = blk(x, rope, st, None)
-        if grow is not None:
-            state.paged.advance(grow)
+            held = self._paged_pass(state, grow, step=not all(live))
+        with held:
+            x = self.embed(tokens)
+            rope = self.rope(tokens.device)
+            for blk, st in zip(self.layers, state.layers):
+                x, _ = blk(x, rope, st, None)
         state.pos += tokens.shape[1]
         return self.final_norm(x)
 
@@ -455,12 +470,11 @@ class Transformer(nn.Module):
         if any(t.dim() != 1 for t in ids):
             raise ValueError("a prompt is one row of tokens")
         flat = torch.cat(ids)[None]
-        state.paged.begin(grow)
-        x = self.embed(flat)
-        rope = self.rope(dev)
-        for blk, st in zip(self.layers, state.layers):
-            x, _ = blk(x, rope, st, None)
-        state.paged.advance(grow)
+        with self._paged_pass(state, grow):
+            x = self.embed(flat)
+            rope = self.rope(dev)
+            for blk, st in zip(self.layers, state.layers):
+                x, _ = blk(x, rope, st, None)
         at, last, slots = 0, [], []
         for b, n in enumerate(grow):
             at += n

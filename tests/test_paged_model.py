@@ -294,3 +294,76 @@ def test_hybrid_and_equal_lengths_over_pages():
         gap = logits.max(-1).values - logits.gather(1, out[:, t:t + 1]).squeeze(1)
         assert float(gap.max()) < 0.15, (t, float(gap.max()))
         logits = eng.model.forward_next_logits_with_state(out[:, t:t + 1], eng.state).float()
+
+
+def _stamp(cache):
+    return (list(cache.held), cache.lengths.tolist(), cache.table.tolist(), [list(p) for p in cache.pages], list(cache.free), cache.rows)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_pass_that_fails_leaves_the_slots_as_they_were(kind):
+    """A token that is none, and a layer that raises: lengths, pages and slots in use are those of before, and what comes then is right."""
+    m = _model("cpu")
+    st, clean = (m.make_paged_state(3, 64, kind, page=16) for _ in range(2))
+    first, second = _prompts([9, 0, 20]), _prompts([30, 5, 0], seed=2)
+    with torch.no_grad():
+        before = _stamp(st.paged)
+        with pytest.raises(IndexError):
+            m.forward_ragged_with_state([[1, 2], None, [3] * 40 + [10 ** 6]], st)
+        assert _stamp(st.paged) == before
+        assert torch.equal(m.forward_ragged_with_state(first, st), m.forward_ragged_with_state(first, clean))
+        before = _stamp(st.paged)
+        for call in (lambda: m.forward_ragged_with_state([[10 ** 6], [1], None], st),
+                     lambda: m.forward_with_state(torch.tensor([[1], [2], [10 ** 6]]), st)):
+            with pytest.raises(IndexError):
+                call()
+            assert _stamp(st.paged) == before
+        assert torch.equal(m.forward_ragged_with_state(second, st), m.forward_ragged_with_state(second, clean))
+        assert _stamp(st.paged) == _stamp(clean.paged)
+        # behind the first layer: its rows are in the pages already, where nobody reads them (in 8 bits they may have moved a page's scale)
+        before = _stamp(st.paged)
+        hook = m.layers[1].register_forward_pre_hook(lambda *_: 1 // 0)
+        with pytest.raises(ZeroDivisionError):
+            m.forward_ragged_with_state(_prompts([3, 3, 14], seed=5), st)
+        hook.remove()
+        assert _stamp(st.paged) == before
+        x, y = (m.forward_next_logits_with_state(torch.tensor([[4], [5], [6]]), s) for s in (st, clean))
+        torch.testing.assert_close(x, y, rtol=0, atol=0 if kind == "paged" else 0.05 * float(y.abs().max()))
+
+
+def test_a_pass_that_fails_leaves_recurrent_layers_as_they_were():
+    cfg = mal.get_builtin_model("hybrid_tiny")
+    cfg.vocab_size = 300
+    torch.manual_seed(0)
+    m = Transformer(cfg).eval()
+    a, b = torch.randint(0, 300, (2, 2, 20))
+    with torch.no_grad():
+        st, clean = m.make_paged_state(2, 64), m.make_paged_state(2, 64)
+        for tok in (a, b):
+            hook = m.layers[-1].register_forward_pre_hook(lambda *_: 1 // 0)
+            with pytest.raises(ZeroDivisionError):
+                m.forward_with_state(tok, st)
+            hook.remove()
+            assert torch.equal(m.forward_with_state(tok, st), m.forward_with_state(tok, clean))
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_captured_decode_that_fails_can_be_called_again(kind, monkeypatch):
+    """The capture behind the first step raises: the lengths are those of before the call, and the same call then gives what it gives alone."""
+    from summa_b200.models import engine
+    eng = InferenceEngine.build(_cfg(4, 2, 128), torch.device("cuda"), quantize=None, init_std=0.05, seed=4)
+    prompts = _prompts([60, 63], seed=3)
+    eng.reset(2, 400, kind)
+    want = eng.decode(eng.prefill_ragged(prompts), 8)
+    eng.reset(2, 400, kind)
+    eng._graph = None
+    first = eng.prefill_ragged(prompts)
+    before = _stamp(eng.state.paged)
+    with monkeypatch.context() as mp:
+        mp.setattr(engine._GraphDecoder, "_capture", lambda *_: 1 // 0)
+        with pytest.raises(ZeroDivisionError):
+            eng.decode(first, 8)
+    assert _stamp(eng.state.paged) == before and eng.state.pos == 0
+    assert torch.equal(eng.decode(first, 8), want)
+    assert eng.state.paged.held == eng.state.paged.lengths.tolist() == [68, 71]
