@@ -346,7 +346,7 @@ static int launch_append(const AppendParams& p, bool one_row, cudaStream_t st) {
     if (np <= 1) paged_append_segments_kernel<D, 1><<<grid, 256, 0, st>>>(p, static_cast<int>(q_blocks));
     else if (np == 2) paged_append_segments_kernel<D, 2><<<grid, 256, 0, st>>>(p, static_cast<int>(q_blocks));
     else if (np <= 4) paged_append_segments_kernel<D, 4><<<grid, 256, 0, st>>>(p, static_cast<int>(q_blocks));
-    else paged_append_segments_kernel<D, 8><<<grid, 256, 0, st>>>(p, static_cast<int>(q_blocks));
+    else if constexpr (PAGED_MAX_PAGE / RPB > 4) paged_append_segments_kernel<D, 8><<<grid, 256, 0, st>>>(p, static_cast<int>(q_blocks));
   }
   SB_CHECK_CUDA(cudaGetLastError());
   return SB_OK;

@@ -355,6 +355,22 @@ def test_append_of_more_rows_than_promised(kind):
     assert torch.equal(kv.v[at, 0, n:].view(torch.uint8), old.v[at, 0, n:].view(torch.uint8))
 
 
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_append_fills_pages_of_every_size(page, D):
+    """Whole pages, and both ends of one, in 8 bits: every number of passes that a block makes over its page."""
+    Hq, Hkv = 2, 2
+    held, rows = [0, page - 3, 5, page // 2], [2 * page, page + 7, 1, page // 4]
+    pr, pages = _rows(held, rows, page, "cuda", max_rows=max(rows))
+    kv = _cache(pages, Hkv, page, D, "e4m3", "cuda")
+    qkv = torch.randn(sum(rows), (Hq + 2 * Hkv) * D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    want_q, want, scales = _exact_append(qkv, None, None, 0.0, None, None, Hq, Hkv, D, kv, pr)
+    q = ops.paged_append(qkv, None, None, 0.0, None, None, Hq, Hkv, D, kv, pr)
+    assert torch.equal(q.cpu().double(), want_q) and _flag() == 0        # (nothing is turned or normed: bf16 as it came)
+    for got, w, s, ws in ((kv.k, want[0], kv.k_scale, scales[0]), (kv.v, want[1], kv.v_scale, scales[1])):
+        assert torch.equal(got.cpu().double(), w) and torch.equal(s.cpu().double(), ws)
+
 # ------------------------------------------------------------------ attention
 
 ATTEND = [
