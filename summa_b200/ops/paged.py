@@ -32,7 +32,7 @@ class PagedRows(NamedTuple):
     anything). `lengths` `[B]` int32: the tokens it had in the cache before the call, negative for a slot that is not in use.
     `starts` `[B + 1]` int32, ascending from 0: sequence b has the rows starts[b] .. starts[b + 1] of the call, and rows behind the last
     belong to nobody; None: one row each. `max_rows`: the most rows of one sequence, which the launch is shaped for (None: the rows of the
-    call); rows beyond it may be left out, and are reported in the error word."""
+    call); rows beyond it may be left out, and what is left out is reported in the error word."""
     table: torch.Tensor
     lengths: torch.Tensor
     starts: Optional[torch.Tensor] = None

@@ -577,6 +577,25 @@ def test_more_rows_than_promised():
 
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D,held", [(64, [50]), (128, [50]), (64, [3000, 7, 500]), (128, [3000, 7, 500])])
+def test_the_promised_rows_are_served_whatever_comes_behind_them(D, held, kind):
+    """max_rows too small, by so few columns that they are one group, cut and whole: the promised rows are those of the formula, the others
+    zeros, bit 4 of the error word."""
+    n = [6, 2, 5][:len(held)]
+    pr, pages = _rows(held, n, 16, "cuda", max_rows=2)
+    kv = _cache(pages, 2, 16, D, kind, "cuda")
+    q = torch.randn(sum(n), 4, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    got = ops.paged_attention(q, kv, pr)
+    assert _flag() == 4
+    want, size = _exact_attention(q, kv, pr, True, None)
+    at = 0
+    for r in n:
+        _near(got[at:at + 2], want[at:at + 2], size[at:at + 2], kind == "e4m3")
+        assert (got[at + 2:at + r] == 0).all()
+        at += r
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 def test_more_rows_than_promised_in_groups(kind):
     pr, pages = _rows([900, 3], [11, 2], 16, "cuda", max_rows=7)
     kv = _cache(pages, 1, 16, 64, kind, "cuda")
