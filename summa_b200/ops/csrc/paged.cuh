@@ -145,6 +145,9 @@ struct PagedAttentionArgs {
 };
 static_assert(sizeof(PagedAppendArgs) == 14 * 8 + 9 * 8 + 12 * 4 && sizeof(PagedAttentionArgs) == 11 * 8 + 11 * 8 + 14 * 4, "packed by the caller");
 
+// Host: whether all of these may be read or written 16 bytes at a time.
+template <typename... P> inline bool aligned16(const P*... p) { return ((reinterpret_cast<uintptr_t>(p) | ... | 0) & 15) == 0; }
+
 // Host: log2 of a page size, -1 if it is not one that the kernels take.
 inline int page_shift_of(int page) {
   return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1;

@@ -362,6 +362,7 @@ extern "C" int sb_paged_append(const sb::PagedAppendArgs* args) {
   SB_CHECK_ARG((c.D == 64 || c.D == 128) && shift >= 0 && c.Hq > 0 && c.Hkv > 0 && c.T > 0 && c.B > 0 && c.P > 0 && c.num_pages > 0);
   SB_CHECK_ARG(c.ld % 8 == 0 && c.q_ld % 8 == 0 && c.max_rows > 0 && (c.starts != nullptr || c.T == c.B));
   SB_CHECK_ARG((c.k_scale == nullptr) == (c.v_scale == nullptr) && (c.cos == nullptr) == (c.sin == nullptr));
+  SB_CHECK_ARG(aligned16(c.qkv, c.q, c.q_gamma, c.k_gamma, c.cos, c.sin, c.k, c.v));
   SB_CHECK_ARG((c.q_gamma == nullptr) == (c.k_gamma == nullptr) && (c.cos == nullptr || c.max_pos > 0));
   AppendParams p;
   p.batch = PagedBatch{c.table, c.lengths, c.starts, c.table_ld, c.P, c.B, c.T, c.max_rows, shift, c.num_pages};

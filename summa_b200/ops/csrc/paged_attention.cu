@@ -862,6 +862,7 @@ extern "C" int sb_paged_attention(const sb::PagedAttentionArgs* args) {
   const int shift = page_shift_of(c.page);
   SB_CHECK_ARG((c.D == 64 || c.D == 128) && shift >= 0 && c.Hq > 0 && c.Hkv > 0 && c.Hq % c.Hkv == 0 && c.T > 0 && c.B > 0 && c.P > 0 && c.num_pages > 0);
   SB_CHECK_ARG(c.max_rows > 0 && (c.starts != nullptr || (c.T == c.B && c.max_rows == 1)) && (c.k_scale == nullptr) == (c.v_scale == nullptr));
+  SB_CHECK_ARG(aligned16(c.q, c.k, c.v, c.o, c.work) && (c.q_ld | c.q_head | c.o_ld | c.o_head) % 8 == 0);
   SB_CHECK_ARG(c.max_rows <= 48 && c.max_rows * (c.Hq / c.Hkv) <= 48);
   const int groups = (c.max_rows * (c.Hq / c.Hkv) + 15) / 16;
   // places of the list of work in 32 bits, at the shortest unit; a page's stride in 32 bits (unsigned)

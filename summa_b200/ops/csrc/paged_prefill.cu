@@ -778,6 +778,7 @@ extern "C" int sb_paged_prefill(const sb::PagedAttentionArgs* args) {
   const int shift = page_shift_of(c.page);
   SB_CHECK_ARG((c.D == 64 || c.D == 128) && shift >= 0 && c.Hq > 0 && c.Hkv > 0 && c.Hq % c.Hkv == 0 && c.T > 0 && c.B > 0 && c.P > 0 && c.num_pages > 0);
   SB_CHECK_ARG((c.starts != nullptr || c.T == c.B) && (c.k_scale == nullptr) == (c.v_scale == nullptr) && c.scale > 0.f);
+  SB_CHECK_ARG(aligned16(c.q, c.k, c.v, c.o, c.work) && (c.q_ld | c.q_head | c.o_ld | c.o_head) % 8 == 0);
   SB_CHECK_ARG(static_cast<long>(c.T) * c.Hq < (1L << 31) - 256);
   const bool fp8 = c.k_scale != nullptr;
   const long size = fp8 ? 1 : 2;

@@ -24,7 +24,7 @@ BF16 = torch.bfloat16
 
 
 def _rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """2-D row view `[rows, last]` with unit inner stride; copies only when needed."""
+    """2-D row view `[rows, last]` with unit inner stride that begins on 16 bytes; copies only when needed."""
     last = x.shape[-1]
     if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
         return x, x.stride(0)
@@ -44,6 +44,8 @@ def _rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
             rows = x.numel() // last
             return torch.as_strided(x, (rows, last), (rs, 1)), rs
     c = x.contiguous()
+    if c.data_ptr() % 16:                        # (contiguous already: no copy was made)
+        c = c.clone()
     return c.view(-1, last), last
 
 

@@ -647,6 +647,42 @@ def test_strides_and_views(kind, rows):
     assert torch.equal(c[:, ::2], b) and (c[:, 1::2] == 0).all()
 
 
+def test_rows_that_begin_between_16_bytes_are_copied():
+    """What the kernels read 16 bytes at a time: contiguous rows at any element of a buffer."""
+    from summa_b200.ops import cuda_ops
+    buf = torch.arange(2 * 24 + 8, dtype=torch.bfloat16)
+    for i in range(8):
+        x = buf[i:i + 48].view(2, 24)
+        for y in (x, x.view(2, 1, 24), buf[i:i + 44].as_strided((2, 20), (24, 1))):
+            rows, ld = cuda_ops._rows(y)
+            assert rows.data_ptr() % 16 == 0 and rows.stride(0) == ld and torch.equal(rows, y.reshape(2, -1))
+            assert (rows.data_ptr() == y.data_ptr()) == (y.data_ptr() % 16 == 0)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows", [None, [7, 20]])
+def test_inputs_that_begin_between_16_bytes(rows, kind):
+    D, page, Hq, Hkv = 64, 16, 4, 2
+    n = rows or [1, 1]
+    pr, pages = _rows([40, 3], n, page, "cuda", one=rows is None, max_rows=max(n))
+    kv = _cache(pages, Hkv, page, D, kind, "cuda")
+    other = _clone(kv)
+    T, W = sum(n), (Hq + 2 * Hkv) * D
+    cos, sin = _table(64, D, "cuda")
+    qkv = torch.randn(T, W, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    gain = (1 + torch.arange(D, device="cuda") / D)
+
+    def odd(t):
+        return torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape).copy_(t)
+
+    a = ops.paged_append(qkv, gain, gain, 1e-5, cos, sin, Hq, Hkv, D, kv, pr)
+    out = odd(torch.zeros_like(a))
+    assert ops.paged_append(odd(qkv), odd(gain), odd(gain), 1e-5, cos, sin, Hq, Hkv, D, other, pr, out) is out
+    assert torch.equal(out, a) and torch.equal(kv.k.float(), other.k.float()) and torch.equal(kv.v.float(), other.v.float())
+    out = odd(torch.zeros_like(a))
+    assert torch.equal(ops.paged_attention(odd(a), kv, pr, out=out), ops.paged_attention(a, kv, pr)) and _flag() == 0
+
 @gpu
 @pytest.mark.parametrize("rows", [None, [2, 1, 3], [50, 9, 20]])
 def test_captured_and_replayed_on_two_streams(rows):
