@@ -421,7 +421,7 @@ paged_decode_kernel(const PagedAttnParams p) {
       for (int h = 0; h < 2; ++h) {
         const int col = col0 + n * 8 + 2 * t + h;
         const long pos = static_cast<long>(s.len) + col / p.G;
-        clo[n][h] = p.window >= 0 ? static_cast<int>(max(pos - p.window, 0L)) : 0;
+        clo[n][h] = p.window >= 0 ? static_cast<int>(min(max(pos - p.window, 0L), static_cast<long>(s.hi))) : 0;
         chi[n][h] = s.hi;
         if (p.causal) chi[n][h] = static_cast<int>(min(static_cast<long>(s.hi), pos + 1));
         else if (p.window >= 0) chi[n][h] = static_cast<int>(min(static_cast<long>(s.hi), pos + p.window + 1));
@@ -429,7 +429,7 @@ paged_decode_kernel(const PagedAttnParams p) {
       }
     }
     // keys that every column sees
-    const int all_lo = p.window >= 0 ? static_cast<int>(max(static_cast<long>(s.len) + s.rows - 1 - p.window, 0L)) : 0;
+    const int all_lo = p.window >= 0 ? static_cast<int>(min(max(static_cast<long>(s.len) + s.rows - 1 - p.window, 0L), static_cast<long>(s.hi))) : 0;
     const int all_hi = p.causal ? static_cast<int>(min(static_cast<long>(s.hi), s.len + 1L))
                                 : p.window >= 0 ? static_cast<int>(min(static_cast<long>(s.hi), static_cast<long>(s.len) + p.window + 1)) : s.hi;
 

@@ -175,7 +175,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
   if (tl.len >= 0) {
     if (p.causal) hi = static_cast<int>(min(static_cast<long>(hi), static_cast<long>(tl.len) + last_row + 1));
     else if (p.window >= 0) hi = static_cast<int>(min(static_cast<long>(hi), static_cast<long>(tl.len) + last_row + p.window + 1));
-    if (p.window >= 0) lo = static_cast<int>(max(static_cast<long>(tl.len) + first_row - p.window, 0L));
+    // (a length may be anything: behind the last key there is none, whatever 32 bits hold)
+    if (p.window >= 0) lo = static_cast<int>(min(max(static_cast<long>(tl.len) + first_row - p.window, 0L), static_cast<long>(hi)));
   }
   int j0 = lo / PP_KEYS, j1 = (hi + PP_KEYS - 1) / PP_KEYS;       // blocks of keys
   if (hi <= lo) j1 = j0;
@@ -481,7 +482,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     int klo = 0, khi = tl.hi;
     if (p.causal) khi = static_cast<int>(min(static_cast<long>(khi), pos + 1));
     if (p.window >= 0) {
-      klo = static_cast<int>(max(pos - p.window, 0L));
+      klo = static_cast<int>(min(max(pos - p.window, 0L), static_cast<long>(khi)));
       khi = static_cast<int>(min(static_cast<long>(khi), pos + p.window + 1));
     }
     if (!live) khi = 0;

@@ -892,6 +892,35 @@ def test_many_small_weights_under_the_largest_scale(D, n):
     _near(got, want.repeat(B, 1, 1), size.repeat(B, 1, 1), True)
     assert _flag() == 0
 
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [1, 3, 70])
+def test_lengths_at_the_end_of_32_bits(n, kind):
+    """A length far behind the table, up to 2^31 - 1: a row without a window sees what the table holds, one with a window nothing."""
+    D, page, Hq, P = 64, 16, 4, 6
+    kv = _cache(P, 1, page, D, kind, "cuda")
+    table = torch.tensor([[3, 1, 5, 0, 2, 4]], dtype=torch.int32, device="cuda")
+    q = torch.randn(n, Hq, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    starts = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    all_keys = PagedRows(table, torch.tensor([P * page - n], dtype=torch.int32, device="cuda"), starts, n)
+    want, size = _exact_attention(q, kv, all_keys, False, None)
+    for length in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 40, 2 ** 31 - 300):
+        rows = PagedRows(table, torch.tensor([length], dtype=torch.int32, device="cuda"), starts, n)
+        for causal in (True, False):
+            for window in (None, 2 ** 31 - 1, 1000, 5, 0):
+                got = ops.paged_attention(q, kv, rows, causal, window)
+                assert _flag() == 4
+                if window is None:
+                    _near(got, want, size, kind == "e4m3")
+                elif window < 2 ** 31 - 1:
+                    assert (got == 0).all()
+                else:
+                    assert got.isfinite().all()
+        qkv = torch.randn(n, 6 * D).to(torch.bfloat16).cuda()
+        old = _clone(kv)
+        assert (ops.paged_append(qkv, None, None, 0.0, None, None, Hq, 1, D, kv, rows) == 0).all() and _flag() == 4
+        assert torch.equal(kv.k.float(), old.k.float()) and torch.equal(kv.v.float(), old.v.float())
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("rows", [None, [2, 3], [70, 40]])
 def test_a_window_wider_than_32_bits_hold_hides_nothing(rows, device):
