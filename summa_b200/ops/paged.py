@@ -112,6 +112,15 @@ def check(x: torch.Tensor, Hkv: int, D: int, kv: PagedKV, rows: PagedRows) -> La
     return Layout(B, P, page, pages, table_ld, k_page, k_head, v_page, v_head, ks_ld, vs_ld)
 
 
+def check_out(out, shape, x) -> None:
+    if out is None:
+        return
+    if out.shape != shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError(f"out: {list(shape)} of the type and device of the rows")
+    if any(step == 0 and n > 1 for step, n in zip(out.stride(), out.shape)):
+        raise ValueError("several elements of out are one in memory")
+
+
 def check_append(qkv, q_gamma, k_gamma, cos, sin, Hq, Hkv, D, kv, rows, out) -> Layout:
     device = qkv.device
     if qkv.dim() != 2 or Hq < 1 or Hkv < 1 or qkv.shape[1] != (Hq + 2 * Hkv) * D:
@@ -129,8 +138,7 @@ def check_append(qkv, q_gamma, k_gamma, cos, sin, Hq, Hkv, D, kv, rows, out) -> 
             raise ValueError("cos and sin have to begin on 16 bytes")
         if cos.shape[0] < 1:
             raise ValueError("cos, sin: no position")
-    if out is not None and (out.shape != (qkv.shape[0], Hq, D) or out.dtype != qkv.dtype or out.device != device):
-        raise ValueError(f"out: [{qkv.shape[0]}, {Hq}, {D}] of the type and device of the rows")
+    check_out(out, (qkv.shape[0], Hq, D), qkv)
     return check(qkv, Hkv, D, kv, rows)
 
 
@@ -145,8 +153,7 @@ def check_attention(q, kv, rows, window, scale, out) -> Layout:
         raise ValueError(f"window {window}")
     if scale is not None and not 0.0 < scale < math.inf:
         raise ValueError(f"scale {scale}: it has to be positive")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device):
-        raise ValueError(f"out: {list(q.shape)} of the type and device of the rows")
+    check_out(out, q.shape, q)
     return check(q, Hkv, D, kv, rows)
 
 

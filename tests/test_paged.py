@@ -1083,3 +1083,35 @@ def test_no_input_drops_a_gradient(kind, device):
     with torch.no_grad():                                                # (a gradient that nobody asks for is none)
         want = attend()
         assert torch.equal(attend(kv=kv._replace(**{n: leaf(getattr(kv, n)) for n in pages})), want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_output_that_lies_on_itself_is_refused(device):
+    q, kv, pr = _good(device)
+    qkv = torch.randn(2, 8 * 64).to(torch.bfloat16).to(device)
+    one = torch.zeros(1, 4, 64, dtype=torch.bfloat16, device=device)
+    for out in (one.expand(2, 4, 64), one[:, :1].expand(2, 4, 64), one.transpose(0, 1)[:2].expand(2, 4, 64)):
+        with pytest.raises(ValueError, match="one in memory"):
+            ops.paged_attention(q, kv, pr, out=out)
+        with pytest.raises(ValueError, match="one in memory"):
+            ops.paged_append(qkv, None, None, 0.0, None, None, 4, 2, 64, kv, pr, out)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows", [None, [3, 2], [70, 40]])
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_outputs_in_the_place_of_the_inputs(kind, rows, device):
+    """Queries left in the projection they came in, attention rows written over their queries."""
+    D, page, Hq, Hkv = 128, 64, 4, 2
+    n = rows or [1, 1]
+    pr, pages = _rows([600, 9], n, page, device, one=rows is None, max_rows=max(n))
+    kv = _cache(pages, Hkv, page, D, kind, device)
+    other = _clone(kv)
+    cos, sin = _table(800, D, device)
+    qkv = torch.randn(sum(n), (Hq + 2 * Hkv) * D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(device)
+    want_q = ops.paged_append(qkv, None, None, 0.0, cos, sin, Hq, Hkv, D, kv, pr)
+    place = qkv[:, :Hq * D].unflatten(1, (Hq, D))
+    assert ops.paged_append(qkv, None, None, 0.0, cos, sin, Hq, Hkv, D, other, pr, place) is place
+    assert torch.equal(place, want_q) and torch.equal(kv.k.float(), other.k.float()) and torch.equal(kv.v.float(), other.v.float())
+    want = ops.paged_attention(want_q, kv, pr)
+    assert ops.paged_attention(place, kv, pr, out=place) is place and torch.equal(place, want)
