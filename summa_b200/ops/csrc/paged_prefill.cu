@@ -152,8 +152,9 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kh = blockIdx.x;
   const PrefillTile tl = prefill_tile(p.batch, p.G, blockIdx.y);
-  // rows behind the last sequence: thread i of n of every CTA
-  auto zero_tail = [&](int i0, int n0) {
+  // rows behind the last sequence: thread i0 of as many in every CTA, with a tile or without (so that together they take all of them)
+  constexpr int n0 = 128;
+  auto zero_tail = [&](int i0) {
     if (!p.zero_tail) return;
     const int t0 = paged_tail(p.batch);
     const long n = static_cast<long>(p.batch.T - t0) * p.Hq * (D / 8);
@@ -165,7 +166,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       *reinterpret_cast<uint4*>(p.o + (t0 + row) * p.o_ld + (x / (D / 8)) * p.o_head + (x % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
     }
   };
-  if (tl.b >= p.batch.B) { zero_tail(threadIdx.x, PP_THREADS); return; }
+  if (tl.b >= p.batch.B) {
+    if (threadIdx.x < n0) zero_tail(threadIdx.x);
+    return;
+  }
 
   // the tile's pairs and the keys that any of them sees
   const unsigned pairs = static_cast<unsigned>(tl.rows) * p.G, x0 = static_cast<unsigned>(tl.tile) * 256, G = p.G;
@@ -360,7 +364,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
         warp_arrive(full(2 * nblk - 1));
       }
     }
-    zero_tail(tid, 128);
+    zero_tail(tid);
   } else if (warp >= 8) {
     // (whole warps go through these loops and one elected thread issues, so that the descriptors, the same for all, stay in uniform
     // registers: from a lane of its own an instruction took 100 cycles to issue)

@@ -541,6 +541,37 @@ def test_rows_behind_the_last_sequence(rows):
 
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("held,rows,behind,max_rows", [([50, 9], [40, 30], 500, None), ([50, -1, 9, 0], [40, 0, 3, 1], 77, None),
+                                                       ([50, 2000], [2, 3], 600, 3), ([700], [1], 4000, 1), ([50, 9], [0, 0], 900, None)])
+def test_many_rows_behind_the_last_sequence_are_zeros(held, rows, behind, max_rows, D, kind):
+    """A call padded far beyond its sequences' rows: all rows behind them are zeros in a fresh output, and as they were in a given one,
+    whatever the memory held."""
+    page, Hq, Hkv = 64, 8, 2
+    pr, pages = _rows(held, rows, page, "cuda", max_rows=max_rows)
+    kv = _cache(pages, Hkv, page, D, kind, "cuda")
+    n = sum(rows)
+    q = torch.randn(n + behind, Hq, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    want, size = _exact_attention(q, kv, pr, True, None)
+    qkv = torch.randn(n + behind, (Hq + 2 * Hkv) * D).to(torch.bfloat16).cuda()
+    for _ in range(3):
+        junk = torch.full_like(q, float("nan"))
+        del junk                                                         # (the memory that the next output gets)
+        got = ops.paged_attention(q, kv, pr)
+        assert (got[n:] == 0).all()
+        if n:
+            _near(got[:n], want[:n], size[:n], kind == "e4m3")
+        out = torch.full_like(q, 3.0)
+        ops.paged_attention(q, kv, pr, out=out)
+        assert (out[n:] == 3).all() and torch.equal(out[:n], got[:n])
+        junk = torch.full_like(q, float("nan"))
+        del junk
+        back = ops.paged_append(qkv, None, None, 0.0, None, None, Hq, Hkv, D, _clone(kv), pr)
+        assert (back[n:] == 0).all() and back.isfinite().all()
+    assert _flag() == 0
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("rows", [None, [40, 2]])
 def test_keys_without_a_page_are_left_out(kind, rows):
     """A page out of range inside a sequence: as if its keys were not there; bit 4 of the error word. A sequence of such pages only: zeros."""
