@@ -166,9 +166,10 @@ def paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv: PagedKV, 
     In 8 bits the rows that this call puts into a page and head need a scale of at least their largest magnitude / 448, as a power of
     two; the page's first slot begins the scale anew, otherwise it only grows, and the codes in front of the rows are then rounded
     to the new one. An infinite or NaN element is stored as NaN and does not count for the scale. Rows of a slot that is not in use store
-    nothing and return zeros; rows behind the last sequence are zeros, or as they were in `out`. No two sequences of a call may append
-    to one page. A position without a page (or beyond cos / sin) stores nothing and returns zeros on CUDA, and sets bit 4 of the device's error
-    word (`native.read_error_flag`); on the CPU it raises. No gradients."""
+    nothing and return zeros; rows behind the last sequence are zeros, or as they were in `out` (which may be the queries' own place in
+    `qkv`). No two sequences of a call may append to one page. A position without a page (or beyond cos / sin) stores nothing and returns
+    zeros on CUDA, and sets bit 4 of the device's error word (`native.read_error_flag`); on the CPU it raises. No gradients and no
+    forward-mode derivative: inputs that ask for one are refused."""
     layout = paged.check_append(qkv, q_gamma, k_gamma, cos, sin, Hq, Hkv, D, kv, rows, out)
     _no_gradient("paged_append", qkv, q_gamma, k_gamma, cos, sin, *kv, out)
     if native_enabled(qkv) and D in (64, 128):
@@ -179,10 +180,11 @@ def paged_append(qkv, q_gamma, k_gamma, eps, cos, sin, Hq, Hkv, D, kv: PagedKV, 
 def paged_attention(q, kv: PagedKV, rows: PagedRows, causal=True, window=None, scale=None, out=None):
     """Attention of the rows `[T, Hq, D]` over the paged cache, which holds them already (`paged_append` with the same `rows`): row
     i of sequence b stands at lengths[b] + i and sees its sequence's keys up to there (all of them with `causal=False`), within `window`
-    on either side. Returns `[T, Hq, D]` (in `out` when given); rows that see no key, and those of a slot that is not in use, are
+    on either side. Returns `[T, Hq, D]` (in `out` when given, which may be `q`); rows that see no key, and those of a slot that is not in use, are
     zeros, rows behind the last sequence zeros, or as they were in `out`. Keys without a page are left out on CUDA, and set bit 4 of the
     device's error word; on the CPU they raise. A value that is not finite reaches the rows whose sequence holds it, and no others; within
-    the rows of one call it may also reach those that the mask keeps from it. No gradients."""
+    the rows of one call it may also reach those that the mask keeps from it. No gradients and no forward-mode derivative: inputs that ask
+    for one are refused."""
     layout = paged.check_attention(q, kv, rows, window, scale, out)
     _no_gradient("paged_attention", q, *kv, out)
     if native_enabled(q) and q.shape[2] in (64, 128):

@@ -15,7 +15,8 @@
 //             registers (in 32 bits, rotated) between the maximum and the conversion, so they are read once.
 // Measured at 32 query heads and 8 kv heads of 128 (a call among others of a graph): one token of one sequence 2.4 us, of 64 sequences 2.6 us,
 // which is what a launch takes; 8 prompts of 2048 rows 77 us into e4m3 and 69 into bf16 pages (4.8 and 5.9 TB/s), 7 of 130 to 2048 into
-// e4m3 28 us (4.3 TB/s). The 8-bit form is bound by issue (67% of the slots): the conversions, and a maximum over every row.
+// e4m3 28 us (4.3 TB/s). The 8-bit form is bound by issue (61% of the slots): the conversions, and a maximum over every row. A single row that
+// raises its page's scale waits for the codes before it: one sequence's 2.3 us become 6 in the middle of a page of 64 and 10 at its end.
 #include "paged.cuh"
 
 namespace sb {

@@ -27,9 +27,9 @@
 // reference that only moves when a score passes it by that), and goes into the product as w 2^11, where f16 has 25 binary orders of
 // full precision below 1 and ten more of less. bf16 pages: w = 2^(s - M) in bf16, as the rows of a bf16 product must be.
 //
-// Measured at 32 query heads over 8 kv heads of 128: 64 sequences of 37 to 8191 tokens in e4m3 43.0 us (4.8 TB/s), one of 100,003 40.2 us
-// (5.1 TB/s; 6.5 over what more tokens add), 12 of up to 16,000 with a window of 4096 in bf16 37.6 us (5.0 TB/s); one of 501 8.0 us. Beside
-// the stream there are some 3.5 us until the first products (the batch's description, the pages, the first tiles) and 2 to 4 of the
+// Measured at 32 query heads over 8 kv heads of 128, pages from memory: 64 sequences of 37 to 8191 tokens in e4m3 43.1 us (4.8 TB/s), one of
+// 100,003 40.0 us (5.1 TB/s; 6.5 over what more tokens add), 12 of up to 16,000 with a window of 4096 in bf16 36.7 us (5.1 TB/s); one of 501
+// 8.1 us. Beside the stream there are some 3.5 us until the first products (the batch's description, the pages, the first tiles) and 2 to 4 of the
 // second kernel. Eight warps with tiles of 16 keys, three CTAs per SM with two stages and joining by the last CTA to arrive (58 us for
 // 43) were slower or no faster.
 #include "paged.cuh"

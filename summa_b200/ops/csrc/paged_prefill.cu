@@ -21,16 +21,18 @@
 // same units), and with e4m3 the warps that expand the codes. Both groups on 16 warps of half a row each were slower (125 to 180 us where
 // this took 102 to 118), and so was fetching two blocks of codes ahead in registers (117 us for 105).
 //
-// Measured at 32 query heads over 8 kv heads of 128: a chunk of 512 rows behind 7500 tokens 105 us in e4m3 and 88 in bf16 pages (621 and
-// 735 TFLOP/s), 256 rows behind 16000 tokens with 37 kv heads, a tile for every SM, 450 and 344 us (694 and 911); six prompts of 200 to 2048
-// rows 104 us, 16 rows behind 4000 tokens 21.
+// Measured at 32 query heads over 8 kv heads of 128: a chunk of 512 rows behind 7500 tokens 105 us in e4m3 and 88 in bf16 pages (619 and
+// 737 TFLOP/s) that lie in the L2 cache, 116 and 89 from memory: e4m3 codes are asked for one block ahead, in registers, bf16 ones two by
+// asynchronous copies. 256 rows behind 16000 tokens with 37 kv heads, a tile for every SM, 457 and 400 us (685 and 780); six prompts of
+// 200 to 2048 rows in bf16 105 us, 16 rows behind 4000 tokens in e4m3 20.5.
 //
 // (A bulk tensor copy could fetch bf16 pages, but not expand codes, nor leave out single rows of a page that hold nothing yet: what
 // lies behind a sequence's last row may be NaN, and 0 * NaN would reach its sums.)
 //
 // 8 bits: as in paged_attention.cu, codes enter the products as f16, a query row scaled by a power of two to at most 2^15, the key
 // scale of each 16 keys in the factor of the scores, the value scale 2^e in the weight w = 2^(s + e - M), beside the sum of 2^(s - M),
-// which is that of w 2^-e. With bf16 pages the factor is the softmax scale and e is 0. Keys that a sequence has no page for have e = -infinity.
+// which is that of w 2^-e, or comes from the scores where pages lie far apart. With bf16 pages the factor is the softmax scale and e is 0.
+// Keys that a sequence has no page for have a score of -infinity.
 //
 // With few tiles the keys are split too: each of `splits` CTAs takes a part of the tile's blocks and leaves O (unnormalised, 32
 // bits), M and l; a second kernel adds them up in order. (Dealing out equal stretches of all tiles' blocks to one CTA per SM instead, the
