@@ -31,7 +31,8 @@
 //
 // 8 bits: as in paged_attention.cu, codes enter the products as f16, a query row scaled by a power of two to at most 2^15, the key
 // scale of each 16 keys in the factor of the scores, the value scale 2^e in the weight w = 2^(s + e - M), beside the sum of 2^(s - M),
-// which is that of w 2^-e, or comes from the scores where pages lie far apart. With bf16 pages the factor is the softmax scale and e is 0.
+// which is that of w 2^-e, or comes from the scores where pages lie far apart. With bf16 pages the factor is the softmax scale, e is
+// 0, and the weights are rounded to bf16, since both operands of a product have one type and the values are bf16.
 // Keys that a sequence has no page for have a score of -infinity.
 //
 // With few tiles the keys are split too: each of `splits` CTAs takes a part of the tile's blocks and leaves O (unnormalised, 32
