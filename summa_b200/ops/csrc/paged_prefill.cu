@@ -10,6 +10,8 @@
 //                     row, through shared memory
 //   warp 8            issues S = Q K^T
 //   warp 9            issues O += P V
+//   warp 10           brings the scales of a block's pages, and says whether they lie far apart (that said by the softmax threads, and the scales
+//                     brought by a copying warp: 107, and 113 from memory, were 106 and 117)
 //   warps 12-15       bring keys and values from their pages into the swizzled tiles that the products read: bf16 as 16-byte
 //                     asynchronous copies, e4m3 through registers, where it becomes f16
 // Tensor memory holds the two groups' O (256 columns), one buffer of 64 scores and two of packed weights each. The scores' buffer is free
@@ -21,10 +23,10 @@
 // same units), and with e4m3 the warps that expand the codes. Both groups on 16 warps of half a row each were slower (125 to 180 us where
 // this took 102 to 118), and so was fetching two blocks of codes ahead in registers (117 us for 105).
 //
-// Measured at 32 query heads over 8 kv heads of 128: a chunk of 512 rows behind 7500 tokens 105 us in e4m3 and 88 in bf16 pages (619 and
-// 737 TFLOP/s) that lie in the L2 cache, 116 and 89 from memory: e4m3 codes are asked for one block ahead, in registers, bf16 ones two by
-// asynchronous copies. 256 rows behind 16000 tokens with 37 kv heads, a tile for every SM, 457 and 400 us (685 and 780); six prompts of
-// 200 to 2048 rows in bf16 105 us, 16 rows behind 4000 tokens in e4m3 20.5.
+// Measured at 32 query heads over 8 kv heads of 128: a chunk of 512 rows behind 7500 tokens 107 us in e4m3 and 88 in bf16 pages (606 and
+// 740 TFLOP/s) that lie in the L2 cache, 113 and 89 from memory: e4m3 codes are asked for one block ahead, in registers, bf16 ones two by
+// asynchronous copies. 256 rows behind 16000 tokens with 37 kv heads, a tile for every SM, 450 and 400 us (694 and 780); six prompts of
+// 200 to 2048 rows in bf16 105 us, 16 rows behind 4000 tokens in e4m3 20.7.
 //
 // (A bulk tensor copy could fetch bf16 pages, but not expand codes, nor leave out single rows of a page that hold nothing yet: what
 // lies behind a sequence's last row may be NaN, and 0 * NaN would reach its sums.)
@@ -144,13 +146,13 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
   uint64_t* s_free = bars + 3;    // [2], 4 arrivals: the group has its scores in registers
   uint64_t* p_full = bars + 5;    // [2][2 buffers], 4 arrivals
   uint64_t* o_full = bars + 9;    // [2][2] the product with a buffer's weights is complete (one for each buffer: who waits is a phase behind at most)
-  uint64_t* k_full = bars + 13;   // [NS], 4 arrivals
+  uint64_t* k_full = bars + 13;   // [NS], 5 arrivals: the keys', and their scales'
   uint64_t* k_empty = bars + 17;
   uint64_t* v_full = bars + 21;   // [NS], 4 arrivals
   uint64_t* v_empty = bars + 25;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float4* scales = reinterpret_cast<float4*>(smem + C::OFF_SCALE);       // [RING][4]: key factor, e, 2^(PAGED_SUM - e)
+  float4* scales = reinterpret_cast<float4*>(smem + C::OFF_SCALE);       // [RING][4]: key factor, e, 2^(PAGED_SUM - e), whether the block's pages are far apart
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kh = blockIdx.x;
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     for (int s = 0; s < 4; ++s) { mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(&s_full[a], 1); mbar_init(&s_free[a], 4); }
     for (int s = 0; s < NS; ++s) {
-      mbar_init(&k_full[s], 4); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 4); mbar_init(&v_empty[s], 1);
+      mbar_init(&k_full[s], 5); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 4); mbar_init(&v_empty[s], 1);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -222,10 +224,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     const uint32_t lane_off = (r0 - group0) * ROWB + c * 16;
     const uint8_t *kb = p.k + kh * p.k_head + lane_off, *vb = p.v + kh * p.v_head + lane_off;
     const unsigned pages = p.batch.num_pages;
-    int id[IDS], next[IDS], group_next = -2;    // (group_next: of group tid, for the scales)
+    int id[IDS], next[IDS];
     auto look_up = [&](int j) {
-      group_next = -2;
-      if (tid < 4 && j < j1 && j * PP_KEYS + tid * 16 + 16 > lo && j * PP_KEYS + tid * 16 < hi) group_next = table[(j * PP_KEYS + tid * 16) >> shift];
 #pragma unroll
       for (int i = 0; i < IDS; ++i) {
         const int key = j * PP_KEYS + i * IDROWS + group0;
@@ -265,29 +265,9 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
     };
     // where elements 8 e .. 8 e + 7 of row r lie in a tile: 64 elements a row of a swizzled half
     auto place = [&](int r, int e) -> uint32_t { return (e >> 3) * (PP_KEYS * 128) + r * 128 + (((e & 7) ^ (r & 7)) << 4); };
-    // The scales of a block's groups of 16 keys, read by the softmax threads behind S: asked for when its pages are known, put down with
-    // its keys. By four threads, each for a group.
-    float4 scale = make_float4(1.f, 0.f, 0.f, 0.f);
-    auto ask_scales = [&](int page) {
-      const bool good = static_cast<unsigned>(page) < pages;
-      if (!good && page != -2) atomicOr(p.err, 4u);
-      scale.z = good ? 1.f : 0.f;
-      if (FP8 && good) { scale.x = p.ks[page * p.ks_ld + kh]; scale.y = p.vs[page * p.vs_ld + kh]; }
-    };
-    auto put_scales = [&](int i) {
-      if (tid < 4) {
-        float4 f = scale;
-        if (FP8) {
-          const int e = min(max(scale_exp(scale.y), PAGED_LEAST_EXP), PAGED_MOST_EXP);
-          f = f.z != 0.f ? make_float4(scale.x, static_cast<float>(e), exp_scale(PAGED_SUM - e), 0.f) : make_float4(1.f, 0.f, 0.f, 0.f);
-        }
-        scales[(i % C::RING) * 4 + tid] = f;
-      }
-    };
     auto turn = [&](int j) {                     // to block j
 #pragma unroll
       for (int x = 0; x < IDS; ++x) id[x] = next[x];
-      if (tid < 4) ask_scales(group_next);
       look_up(j + 1);
     };
     bool ok = true;
@@ -323,7 +303,6 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       for (int i = 0; i < nblk && ok; ++i) {
         const int s = i % NS;
         load(rv, vb, p.v_page, j0 + i);
-        put_scales(i);
         ok = mbar_wait(&k_empty[s], ((i / NS) & 1) ^ 1, abort_flag, p.err);
         if (!ok) break;
         store(rk, smem + C::OFF_K + s * C::KTILE);
@@ -341,10 +320,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       for (int n = 0; n < 2 * nblk && ok; ++n) {
         const int i = n >> 1, j = j0 + i, s = i % NS;
         const bool is_v = n & 1;
-        if (!is_v) {
-          turn(j);
-          put_scales(i);
-        }
+        if (!is_v) turn(j);
         ok = mbar_wait(is_v ? &v_empty[s] : &k_empty[s], ((i / NS) & 1) ^ 1, abort_flag, p.err);
         if (!ok) break;
         uint8_t* dst = smem + (is_v ? C::OFF_V : C::OFF_K) + s * C::KTILE;
@@ -420,6 +396,39 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
           __syncwarp();
         }
       }
+    } else if (warp == 10 && nblk > 0) {
+      // -------------------------------------------------------------- scales
+      // Of a block's groups of 16 keys, read by the softmax threads behind S: a lane for each group. Short of 2^100 between the scales of a
+      // block's pages and those in front of them a share of the sum l down to 2^-25 of the largest has a weight of 2^(e - the largest e - 16) or
+      // more, which 32 bits hold; a block with a page further below the largest so far is marked.
+      const int* table = p.batch.table + tl.b * p.batch.table_ld;
+      const unsigned pages = p.batch.num_pages;
+      auto look_up = [&](int j) {                // -2: no key of the sequence; others out of range: no page
+        const int key = j * PP_KEYS + lane * 16;
+        return lane < 4 && j < j1 && key + 16 > lo && key < hi ? table[key >> p.batch.page_shift] : -2;
+      };
+      int id = look_up(j0), top_e = PAGED_LEAST_EXP;
+      bool ok = true;
+      for (int i = 0; i < nblk && ok; ++i) {
+        const int page = id;
+        const bool good = static_cast<unsigned>(page) < pages;
+        id = look_up(j0 + i + 1);
+        if (!good && page != -2) atomicOr(p.err, 4u);
+        float4 f = make_float4(1.f, 0.f, good ? 1.f : 0.f, 0.f);
+        if (FP8) {
+          float vs = 1.f;
+          if (good) { f.x = p.ks[page * p.ks_ld + kh]; vs = p.vs[page * p.vs_ld + kh]; }
+          const int e = min(max(scale_exp(vs), PAGED_LEAST_EXP), PAGED_MOST_EXP);
+          const int least = __reduce_min_sync(0xffffffffu, good ? e : PAGED_MOST_EXP);
+          top_e = max(top_e, __reduce_max_sync(0xffffffffu, good ? e : PAGED_LEAST_EXP));
+          if (good) { f.y = static_cast<float>(e); f.z = exp_scale(PAGED_SUM - e); }
+          f.w = least + 100 < top_e ? 1.f : 0.f;
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[i % NS], ((i / NS) & 1) ^ 1, abort_flag, p.err));
+        if (!ok) break;
+        if (lane < 4) scales[(i % C::RING) * 4 + lane] = f;
+        warp_arrive(&k_full[i % NS]);
+      }
     }
     __syncwarp();
   } else {
@@ -493,7 +502,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       khi = static_cast<int>(min(static_cast<long>(khi), pos + p.window + 1));
     }
     if (!live) khi = 0;
-    float m_ref = -INFINITY, l = 0.f, top_e = -INFINITY;          // top_e: the largest exponent of a page's scale so far
+    float m_ref = -INFINITY, l = 0.f;
     bool ok = a < tiles_here;
 #pragma unroll 1
     for (int i = 0; i < nblk && ok; ++i) {
@@ -564,10 +573,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) paged_prefill_kernel(const Page
       }
       const float nm = C::HEAD - (m_ref == -INFINITY ? 0.f : m_ref);
       if (FP8) {
-        // Of pages far apart in scale the one's w is nothing beside the other's, its share of l is not: behind a page 2^100 above, l comes from
-        // the scores. Short of that a share down to 2^-25 of the largest has a w of 2^(e - the largest e - 16) or more, which 32 bits hold.
-        top_e = fmaxf(fmaxf(top_e, fmaxf(e[0], e[1])), fmaxf(e[2], e[3]));
-        if (__builtin_expect(fminf(fminf(e[0], e[1]), fminf(e[2], e[3])) + 100.f < top_e, 0)) {
+        // (of pages far apart in scale the one's w is nothing beside the other's, its share of l is not: then l comes from the scores)
+        float apart;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(apart) : "r"(sc + 12) : "memory");
+        if (__builtin_expect(apart != 0.f, 0)) {
 #pragma unroll
           for (int k = 0; k < 64; ++k) l += inv[k >> 4] != 0.f ? fast_exp2(fmaf(__uint_as_float(v[k]), fs[k >> 4], nm + PAGED_SUM)) : 0.f;
           inv[0] = inv[1] = inv[2] = inv[3] = 0.f;
